@@ -2,8 +2,9 @@
 reduction path -- RMSNorm (+ fused residual add), interleaved GQA RoPE,
 SwiGLU, masked row softmax and the GGUF Q4_0 token-embedding gather -- and,
 beside them, the dequant-GEMV and row dequant for GGUF Q4_0 / Q8_0 / Q4_K /
-Q6_K weights, GQA decode attention, GGUF and .nvmw model files and the
-decode engine that runs them all per token.
+Q6_K weights, GQA decode attention (of one token, or of a tree of drafted
+ones), bounded KV caches, GGUF and .nvmw model files and the decode engine that
+runs them all per token.
 
 The kernels live in libjinf_hip.so behind the C-ABI of include/jinf/*.h;
 this package is a thin ctypes/torch front end used by tests and bench.py.
@@ -42,6 +43,16 @@ from .ops import (  # noqa: F401
     rope_rows,
     softmax_rows,
     swiglu,
+)
+from .kv import (  # noqa: F401,E402
+    attention_decode_scored,
+    attention_scored_workspace,
+    attention_tree,
+    attention_tree_workspace,
+    cache_append,
+    cache_evict,
+    cache_evict_workspace,
+    tree_mask,
 )
 from . import gguf  # noqa: F401,E402
 from . import nvmw  # noqa: F401,E402

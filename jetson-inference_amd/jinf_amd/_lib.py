@@ -26,6 +26,7 @@ Q4_0, Q8_0, Q4_K, Q6_K = 2, 8, 12, 14
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_int64
 
 # name -> (restype, argtypes); the parameter lists of the C declarations.
 SIGNATURES = {
@@ -75,6 +76,18 @@ SIGNATURES = {
     "jinf_rmsnorm_qkv_rope_batch": (_I, [_P, _P, _P, _I, _P, _I, _P, _I, _F, _I, _P, _I, _P,
                                          _P, _I, ctypes.c_int64, _P, _I, _I, _I, _I, _F, _I,
                                          _P, ctypes.c_size_t, _P]),
+    # drafted tokens and bounded caches (include/jinf/kv/kv_hip.h)
+    "jinf_attention_tree": (_I, [_P, _I, _L, _P, _I, _L, _P, _P, _I, _L, _L, _P, _P, _P, _I, _I, _L,
+                                 _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, ctypes.c_size_t, _P]),
+    "jinf_attention_tree_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "jinf_attention_decode_scored": (_I, [_P, _I, _P, _I, _P, _P, _I, _L, _L, _P, _L, _L, _P, _I,
+                                          _I, _I, _I, _I, _F, _P, ctypes.c_size_t, _P]),
+    "jinf_attention_scored_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
+    "jinf_cache_append": (_I, [_P, _P, _I, _L, _L, _P, _L, _L, _P, _P, _P, _P, _I, _I, _L, _I, _P,
+                               _P, _I, _I, _I, _I, _I, _P]),
+    "jinf_cache_evict": (_I, [_P, _P, _L, _L, _P, _P, _I, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P,
+                              _P, _I, _I, _I, _I, _I, _I, _I, _P, ctypes.c_size_t, _P]),
+    "jinf_cache_evict_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),
     # bandwidth probes (include/jinf/probe_hip.h)
     "jinf_probe_rows_inplace": (_I, [_P, ctypes.c_int64, _I, _P, ctypes.c_int64, _I, _I, _I,
                                      _I, _P]),
