@@ -28,8 +28,13 @@ struct TreeArgs {
     float c;  // scale * log2(e)
     float* scores;  // null, or the scores [n_seq][n_heads][ld_scores] wanted
     int64_t ld_scores;
-    float* records;  // {O[head_dim], m, l} per (sequence, row, chunk), or null
     int draft_f16;
+    // Contexts in chunks of `chunk` positions, nch of them at most; chunk 0 also
+    // takes the drafted tokens.  Row (s, j, r) chunk c has its partial sums at
+    // part[((s n_kv + j) rows + r) nch + c][head_dim] and {m, l} at stats[same].
+    int chunk, nch;
+    float* part;
+    float2* stats;
 };
 
 __device__ __forceinline__ float tree_exp2(float a) { return __builtin_amdgcn_exp2f(a); }
@@ -109,27 +114,543 @@ __global__ __launch_bounds__(64) void tree_any_kernel(TreeArgs a) {
         const int d = lane + e * kWave;
         if (d < hd) oh[d] = n > 0 ? acc[e] / l : 0.0f;
     }
-    if (a.records && lane == 0) {
-        float* rec = a.records + ((int64_t)s * a.n_heads + h) * (hd + 2);
-        rec[hd] = m;
-        rec[hd + 1] = l;
+    if (a.stats && lane == 0) a.stats[(int64_t)s * a.n_heads + h] = make_float2(m, l);
+}
+
+// ---- head_dim 64 and 128: matrix cores ----
+//
+// Per tile of positions, with the rows (node, head) of one kv head as columns:
+//   S^T[t][r]  = sum_d K[t][d] Q'[d][r]       Q' = c q
+//   O^T[d][r] += sum_t V^T[d][t] P'^T[t][r]   P' = 2^15 2^(S - m)
+// Both products leave row r in lane r % 16 of every lane group, so the running
+// maximum, the sum and the rescaling of O are one value a lane, and the scores'
+// accumulators are the second product's operand as they stand.  The 2^15 keeps
+// the probabilities of an fp16 product in its normal range; the sum l carries it
+// too, so it cancels.
+//   fp16 cache: v_mfma_f32_16x16x32_f16, Q' and P' as fp16 hi + lo in two products
+//   into one accumulator (about 22 bits); V^T through transposing LDS reads.
+//   fp32 cache: v_mfma_f32_16x16x4_f32, exact products.
+//
+// What bounds it: the K and V bytes while a kv head has few rows, the matrix
+// cores and the softmax's vector work from about 64 rows on.  A workgroup's 4
+// waves therefore share out rows and positions: RW waves take 16 R rows each,
+// and 4 / RW groups of them the positions of a tile; every wave reads a tile's K
+// and V from LDS once for its 16 R rows.
+typedef _Float16 tr_h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 tr_h8 __attribute__((ext_vector_type(8)));
+typedef float tr_f4 __attribute__((ext_vector_type(4)));
+typedef float tr_f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef short tr_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) tr_s4 tr_lds_s4;
+
+__device__ __forceinline__ tr_h8 tr_cat(tr_h4 a, tr_h4 b) {
+    return tr_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// x as fp16 hi and lo parts, four at a time.
+// Of products: the conversion is kept apart from the multiply (f2h2), which the
+// compiler otherwise merges into one instruction of another rounding for hi, but
+// not for the hi that lo is the rest of.
+__device__ __forceinline__ void tr_split_product(const float (&x)[4], tr_h4& hi, tr_h4& lo) {
+    hi = __builtin_bit_cast(tr_h4, make_uint2(f2h2(x[0], x[1]), f2h2(x[2], x[3])));
+    lo = __builtin_bit_cast(tr_h4, make_uint2(f2h2(x[0] - (float)hi[0], x[1] - (float)hi[1]),
+                                              f2h2(x[2] - (float)hi[2], x[3] - (float)hi[3])));
+}
+// Of exponentials: plain conversions, since an instruction in inline assembly must
+// not read v_exp's result without the wait that the compiler places for its own.
+__device__ __forceinline__ void tr_split_exp(const float (&x)[4], tr_h4& hi, tr_h4& lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        hi[i] = (_Float16)x[i];
+        lo[i] = (_Float16)(x[i] - (float)hi[i]);
     }
 }
 
+template <typename TC, int HD, int R_, int RW_>
+struct TreeShape {
+    static constexpr bool F16 = sizeof(TC) == 2;
+    static constexpr int R = R_, RW = RW_, PW = 4 / RW_;
+    static constexpr int ROWS = 16 * R * RW;               // rows per workgroup
+    static constexpr int ST = F16 ? (RW == 4 ? 64 : 128) : (RW == 4 ? 32 : 64);  // positions per tile
+    static constexpr int TP = ST / PW;                     // of them, a wave's
+    static constexpr int PITCH = HD * (int)sizeof(TC);     // LDS bytes per row
+    static constexpr int CH = PITCH / 16;                  // 16-byte pieces per row
+    static constexpr int LD = ST * CH / 256;               // loads per lane per tile (K or V)
+    static constexpr int BUF = 2 * ST * PITCH;             // K tile, V tile
+    static constexpr int MERGE = PW > 1 ? PW * ROWS * (HD + 4) * 4 : 0;
+    static constexpr int LDS = 2 * BUF > MERGE ? 2 * BUF : MERGE;
+    static constexpr int WGS = 2 * LDS <= 160 * 1024 ? 2 : 1;  // workgroups per CU
+};
+
+// LDS place of a row's 16-byte piece c.  K: the 16 rows that a fragment read
+// touches at one piece lie in distinct banks; V: so do the rows of a lane group's
+// transposing read (fp16), and the rows 4 apart of a wave's read (fp32).
+template <typename TC, int HD>
+__device__ __forceinline__ int tree_k_at(int r, int c) {
+    return c ^ (sizeof(TC) == 2 && HD == 64 ? (r >> 1) & 7 : r & 15);
+}
+template <typename TC>
+__device__ __forceinline__ int tree_v_at(int r, int c) {
+    return c ^ (sizeof(TC) == 2 ? 2 * (r & 3) : 4 * ((r >> 2) & 3));
+}
+
+// grid (row tiles * n_kv, n_seq, chunks), 256 threads; the kv head is the fastest
+// index, so that row tiles of one head, which read the same K and V, lie n_kv
+// apart (on one XCD for 8 kv heads).
+template <typename TC, int HD, int R, int RW>
+__global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfma_kernel(TreeArgs a) {
+    using Sh = TreeShape<TC, HD, R, RW>;
+    constexpr bool F16 = Sh::F16;
+    constexpr int PW = Sh::PW, ST = Sh::ST, TP = Sh::TP, PITCH = Sh::PITCH, CH = Sh::CH, LD = Sh::LD;
+    constexpr int NBK = TP / 16;   // 16-position blocks of a wave's part of a tile
+    constexpr int NB = HD / 16;    // 16-dim blocks of the output
+    constexpr int QV = F16 ? HD / 32 : HD / 4;  // q registers: h8 (hi and lo each) or floats
+    extern __shared__ __attribute__((aligned(16))) uint8_t tree_lds[];
+    __shared__ unsigned s_bad[4];  // drafted rows of the tile whose V has a non-finite value
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+    const int col = lane & 15, lg = lane >> 4;
+    const int pw = wave / RW, rw = wave % RW;
+    const int j = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv, s = blockIdx.y, cix = blockIdx.z;
+    const int len = min(max(a.lens[s], 0), a.max_ctx);
+    const int nodes = a.n_nodes ? min(max(a.n_nodes[s], 0), a.max_nodes) : a.max_nodes;
+    const int rows = nodes * a.group, all_rows = a.max_nodes * a.group;
+    const int row0 = tile * Sh::ROWS;
+    const int c0 = cix * a.chunk, c1 = min(len, c0 + a.chunk);
+    if (row0 >= rows || (cix > 0 && c0 >= len)) return;  // (workgroup-uniform, before any barrier)
+    const int used = max(1, (len + a.chunk - 1) / a.chunk);
+    const int drafts = a.mask && cix == 0 ? nodes : 0;
+    const int n_dt = (drafts + ST - 1) / ST;
+    const int n_it = n_dt + (max(c1 - c0, 0) + ST - 1) / ST;
+
+    const char* kb = reinterpret_cast<const char*>(static_cast<const TC*>(a.kc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const TC*>(a.vc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
+    const uint32_t rowb = (uint32_t)a.ld_pos * (uint32_t)sizeof(TC);  // (the host keeps ST of them below 2^31)
+    uint32_t koff[LD], voff[LD];
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+        const int slot = tid + 256 * i, r = slot / CH, p = slot % CH;
+        koff[i] = (uint32_t)r * rowb + 16u * (uint32_t)tree_k_at<TC, HD>(r, p);
+        voff[i] = (uint32_t)r * rowb + 16u * (uint32_t)tree_v_at<TC>(r, p);
+    }
+    // Positions t0 .. of the cache straight to LDS; rows at or past c1 read as zeros.
+    auto load_cached = [&](int t0, int buf) {
+        const int64_t at = (int64_t)t0 * rowb;
+        const int nrec = (int)((uint32_t)min(ST, c1 - t0) * rowb);
+        const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(kb + at), (short)0, nrec, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(vb + at), (short)0, nrec, 0x00020000);
+        uint8_t* base = tree_lds + buf * Sh::BUF + 1024 * wave;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) lds_load16_buf(krs, koff[i], 0, base + 4096 * i);
+#pragma unroll
+        for (int i = 0; i < LD; ++i) lds_load16_buf(vrs, voff[i], 0, base + ST * PITCH + 4096 * i);
+    };
+    // Drafted tokens d0 .. as the cache would hold them; tokens past the sequence's
+    // read as zeros, and so do non-finite V values (noted in s_bad, set up by the
+    // caller): their probability is 0 in rows that do not see them, their product not.
+    constexpr int EL = 16 / (int)sizeof(TC);  // elements per 16-byte piece
+    const int64_t dbase = (int64_t)s * a.ld_draft_seq + (int64_t)j * HD;
+    auto load_draft = [&](int d0, int buf) {
+        uint8_t* base = tree_lds + buf * Sh::BUF;
+#pragma unroll 1
+        for (int i = 0; i < 2 * LD; ++i) {
+            const bool is_v = i >= LD;
+            const int slot = tid + 256 * (is_v ? i - LD : i), r = slot / CH, p = slot % CH;
+            const int c = is_v ? tree_v_at<TC>(r, p) : tree_k_at<TC, HD>(r, p);
+            float e[EL] = {};
+            if (d0 + r < drafts) {
+                const int64_t at = dbase + (int64_t)(d0 + r) * a.ld_draft + (int64_t)c * EL;
+                const void* src = is_v ? a.vd : a.kd;
+                bool bad = false;
+#pragma unroll
+                for (int x = 0; x < EL; ++x) {
+                    const float f = tree_draft<TC>(src, a.draft_f16, at + x);
+                    const bool nf = is_v && !(fabsf(f) < INFINITY);
+                    bad |= nf;
+                    e[x] = nf ? 0.0f : f;
+                }
+                if (bad) atomicOr(&s_bad[r >> 5], 1u << (r & 31));
+            }
+            *reinterpret_cast<uint4*>(base + (is_v ? ST * PITCH : 0) + slot * 16) = Act<TC>::pack(e);
+        }
+    };
+
+    // The lane's rows, their mask and q
+    int node[R], head[R];
+    bool live[R];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        const int r = row0 + (rw * R + g) * 16 + col;
+        live[g] = r < rows;
+        node[g] = live[g] ? r / a.group : 0;
+        head[g] = j * a.group + (live[g] ? r - node[g] * a.group : 0);
+    }
+    const bool idle = row0 + rw * R * 16 >= rows;  // none of the wave's rows is live
+
+    if (tid < 4) s_bad[tid] = 0u;
+    // A first tile of drafted tokens is read by ordinary loads; the first cached
+    // tile is on its way to the other buffer before them.
+    const bool ahead = n_dt == 1 && n_it > 1;
+    if (n_dt > 0) {
+        if (ahead) load_cached(c0, 1);
+        __syncthreads();  // s_bad
+        load_draft(0, 0);
+    } else if (n_it > 0) {
+        load_cached(c0, 0);
+    }
+
+    tr_h8 qh[R][F16 ? QV : 1], ql[R][F16 ? QV : 1];
+    float qf[R][F16 ? 1 : QV];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        const float* qp = a.q + (int64_t)s * a.ld_q_seq + (int64_t)node[g] * a.ld_q + (int64_t)head[g] * HD;
+        const float cs = live[g] ? a.c : 0.0f;
+        if constexpr (F16) {
+            // 32-deep k-step u: lane group lg holds dims HD / 4 lg + 8 u .. + 7, the
+            // 16-byte piece HD / 32 lg + u of the K row
+#pragma unroll
+            for (int u = 0; u < QV; ++u) {
+                tr_h4 hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float4 v = *reinterpret_cast<const float4*>(qp + HD / 4 * lg + 8 * u + 4 * e);
+                    const float x[4] = {v.x * cs, v.y * cs, v.z * cs, v.w * cs};
+                    tr_split_product(x, hi[e], lo[e]);
+                }
+                qh[g][u] = tr_cat(hi[0], hi[1]);
+                ql[g][u] = tr_cat(lo[0], lo[1]);
+            }
+        } else {
+            // 4-deep k-step 4 u + i: lane group lg holds dim 16 u + 4 lg + i, element i
+            // of the K row's 16-byte piece 4 u + lg
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u) {
+                const float4 v = *reinterpret_cast<const float4*>(qp + 16 * u + 4 * lg);
+                qf[g][4 * u] = v.x * cs, qf[g][4 * u + 1] = v.y * cs;
+                qf[g][4 * u + 2] = v.z * cs, qf[g][4 * u + 3] = v.w * cs;
+            }
+        }
+    }
+
+    float m[R], lsum[R];
+    tr_f4 O[R][NB];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        m[g] = -INFINITY, lsum[g] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) O[g][n] = tr_f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int buf = 0;
+#pragma unroll 1
+    for (int it = 0; it < n_it; ++it, buf ^= 1) {
+        const bool draft = it < n_dt;
+        const int t0 = draft ? it * ST : c0 + (it - n_dt) * ST;
+        // this tile has landed for every wave, and every wave is done with the other buffer
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm<0>());
+        __syncthreads();
+        unsigned long long bad = 0;
+        if (draft) {
+            const int b0 = pw * TP;  // the wave's bits (TP <= 64, within two words)
+            bad = (unsigned long long)s_bad[b0 >> 5] | (TP > 32 ? (unsigned long long)s_bad[(b0 >> 5) + 1] << 32 : 0ull);
+            if constexpr (TP < 32) bad = (bad >> (b0 & 31)) & ((1ull << TP) - 1);
+            __syncthreads();
+            if (tid < 4) s_bad[tid] = 0u;
+            if (it + 1 < n_dt) {
+                __syncthreads();
+                load_draft(t0 + ST, buf ^ 1);
+            }
+        }
+        if (it + 1 >= n_dt && it + 1 < n_it && !(ahead && it == 0))
+            load_cached(c0 + (it + 1 - n_dt) * ST, buf ^ 1);
+        const int p0 = t0 + pw * TP;  // the wave's first position (or drafted token)
+        const int left = (draft ? drafts : c1) - p0;  // live ones from there
+        if (left <= 0 || idle) continue;  // (wave-uniform)
+        const uint8_t* kst = tree_lds + buf * Sh::BUF + pw * TP * PITCH;
+        const uint8_t* vst = kst + ST * PITCH;
+        tr_f4 S[R][NBK];
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+            const int r = 16 * b + col;
+#pragma unroll
+            for (int g = 0; g < R; ++g) S[g][b] = tr_f4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (F16) {
+#pragma unroll
+                for (int u = 0; u < QV; ++u) {
+                    const tr_h8 kf = *reinterpret_cast<const tr_h8*>(
+                        kst + r * PITCH + 16 * tree_k_at<TC, HD>(pw * TP + r, QV * lg + u));
+#pragma unroll
+                    for (int g = 0; g < R; ++g) {
+                        S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g][u], S[g][b], 0, 0, 0);
+                        S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][u], S[g][b], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < HD / 16; ++u) {
+                    const tr_f4 kf = *reinterpret_cast<const tr_f4*>(
+                        kst + r * PITCH + 16 * tree_k_at<TC, HD>(pw * TP + r, 4 * u + lg));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int g = 0; g < R; ++g)
+                            S[g][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[g][4 * u + i], S[g][b], 0, 0, 0);
+                }
+            }
+        }
+        if (draft) {
+            // bit 16 b + 4 lg + r: the lane's row sees drafted token p0 + 16 b + 4 lg + r
+#pragma unroll
+            for (int g = 0; g < R; ++g) {
+                unsigned long long bits = 0;
+                if (live[g]) bits = a.mask[((int64_t)s * a.max_nodes + node[g]) * a.words + (p0 >> 6)] >> (p0 & 63);
+                if (left < 64) bits &= (1ull << left) - 1;
+                bits >>= 4 * lg;
+#pragma unroll
+                for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!((bits >> (16 * b + r)) & 1)) S[g][b][r] = -INFINITY;
+            }
+        } else {
+            if (left < TP) {
+#pragma unroll
+                for (int g = 0; g < R; ++g)
+#pragma unroll
+                    for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (16 * b + 4 * lg + r >= left) S[g][b][r] = -INFINITY;
+            }
+            if (a.scores) {
+#pragma unroll
+                for (int g = 0; g < R; ++g) {
+                    float* sc = a.scores + ((int64_t)s * a.n_heads + head[g]) * a.ld_scores + p0 + 4 * lg;
+#pragma unroll
+                    for (int b = 0; b < NBK; ++b)
+                        if (live[g] && 16 * b + 4 * lg < left)
+                            *reinterpret_cast<tr_f4*>(sc + 16 * b) = S[g][b];
+                }
+            }
+        }
+        tr_h4 ph[R][F16 ? NBK : 1], pl[R][F16 ? NBK : 1];
+#pragma unroll
+        for (int g = 0; g < R; ++g) {
+            float tmax = S[g][0][0];
+#pragma unroll
+            for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, S[g][b][r]);
+            tmax = fmaxf(tmax, __shfl_xor(tmax, 16, kWave));
+            tmax = xor32_max(tmax);
+            if (__ballot(tmax > m[g])) {  // some row's maximum grows: its sums scale down
+                const float mn = fmaxf(m[g], tmax);
+                const float corr = tree_exp2(m[g] - softmax_ref(mn));
+                m[g] = mn;
+                lsum[g] *= corr;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) O[g][n] *= corr;
+            }
+            const float ref = softmax_ref(m[g]) - 15.0f;
+            float psum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NBK; ++b) {
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = tree_exp2(S[g][b][r] - ref);
+                    psum += x[r];
+                }
+                if constexpr (F16) tr_split_exp(x, ph[g][b], pl[g][b]);
+                else S[g][b] = tr_f4{x[0], x[1], x[2], x[3]};
+            }
+            lsum[g] += psum;
+        }
+        if constexpr (F16) {
+            // V^T[16 n + col][16 b + 4 lg + i], i = 0..3, in one transposing read
+            auto vfrag = [&](int b, int n) {
+                const int vr = 16 * b + 4 * lg + (col >> 2);
+                const int p = tree_v_at<TC>(vr, 2 * n + ((col & 3) >> 1));
+                return __builtin_bit_cast(tr_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (tr_lds_s4*)(vst + vr * PITCH + 16 * p + 8 * (col & 1))));
+            };
+#pragma unroll
+            for (int bp = 0; bp < NBK / 2; ++bp)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const tr_h8 v = tr_cat(vfrag(2 * bp, n), vfrag(2 * bp + 1, n));
+#pragma unroll
+                    for (int g = 0; g < R; ++g) {
+                        O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            v, tr_cat(ph[g][2 * bp], ph[g][2 * bp + 1]), O[g][n], 0, 0, 0);
+                        O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            v, tr_cat(pl[g][2 * bp], pl[g][2 * bp + 1]), O[g][n], 0, 0, 0);
+                    }
+                }
+        } else {
+            // k-step r: lane group lg holds position 16 b + 4 lg + r
+#pragma unroll
+            for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int vr = 16 * b + 4 * lg + r;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        const float v = *reinterpret_cast<const float*>(
+                            vst + vr * PITCH + 16 * tree_v_at<TC>(pw * TP + vr, 4 * n + (col >> 2)) + 4 * (col & 3));
+#pragma unroll
+                        for (int g = 0; g < R; ++g)
+                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[g][b][r], O[g][n], 0, 0, 0);
+                    }
+                }
+        }
+        if (bad) {
+            // non-finite V values: NaN in their dims of the rows that see them
+#pragma unroll 1
+            for (unsigned long long left_bad = bad; left_bad; left_bad &= left_bad - 1) {
+                const int d = p0 + __builtin_ctzll(left_bad);
+                const int64_t at = dbase + (int64_t)d * a.ld_draft;
+#pragma unroll
+                for (int g = 0; g < R; ++g) {
+                    if (!live[g] || !((a.mask[((int64_t)s * a.max_nodes + node[g]) * a.words + (d >> 6)] >> (d & 63)) & 1))
+                        continue;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!(fabsf(tree_draft<TC>(a.vd, a.draft_f16, at + 16 * n + 4 * lg + r)) < INFINITY))
+                                O[g][n][r] = NAN;
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        lsum[g] += __shfl_xor(lsum[g], 16, kWave);
+        lsum[g] = xor32_sum(lsum[g]);
+    }
+    const bool direct = used <= 1;
+    // Whether a node sees nothing at all: its outputs are zeros.  (A node whose
+    // scores are all -inf has no sum either, and gets NaN.)
+    auto sees_none = [&](int nd) {
+        if (len > 0) return false;
+        uint64_t any = 0;
+        for (int w = 0; 64 * w < drafts; ++w) {
+            const uint64_t x = a.mask[((int64_t)s * a.max_nodes + nd) * a.words + w];
+            any |= drafts - 64 * w < 64 ? x & ((1ull << (drafts - 64 * w)) - 1) : x;
+        }
+        return any == 0;
+    };
+    // row r's place in the partial sums
+    const int64_t rec0 = ((int64_t)s * a.n_kv + j) * all_rows;
+    auto put = [&](int r, int nd, int hh, int d, tr_f4 o, float M, float L) {
+        if (direct) {
+            float* p = a.out + (int64_t)s * a.ld_out_seq + (int64_t)nd * a.ld_out + (int64_t)hh * HD + d;
+            const bool none = L == 0.0f && sees_none(nd);
+            *reinterpret_cast<tr_f4u*>(p) = none ? tr_f4{0.f, 0.f, 0.f, 0.f} : o / L;
+        } else {
+            *reinterpret_cast<tr_f4*>(a.part + ((rec0 + r) * a.nch + cix) * HD + d) = o;
+        }
+        if (d == 0 && a.stats) a.stats[(rec0 + r) * a.nch + cix] = make_float2(M, L);
+    };
+    if constexpr (PW == 1) {
+#pragma unroll
+        for (int g = 0; g < R; ++g) {
+            if (!live[g]) continue;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                put(row0 + (rw * R + g) * 16 + col, node[g], head[g], 16 * n + 4 * lg, O[g][n], m[g], lsum[g]);
+        }
+    } else {
+        // the position groups' states through LDS, merged in their order
+        constexpr int MS = HD + 4;
+        float* mg = reinterpret_cast<float*>(tree_lds);
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < R; ++g) {
+            float* e = mg + (pw * Sh::ROWS + (rw * R + g) * 16 + col) * MS;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) *reinterpret_cast<tr_f4*>(e + 16 * n + 4 * lg) = O[g][n];
+            if (lg == 0) e[HD] = m[g], e[HD + 1] = lsum[g];
+        }
+        __syncthreads();
+        for (int x = tid; x < Sh::ROWS * (HD / 4); x += 256) {
+            const int rl = x / (HD / 4), d = x % (HD / 4) * 4;
+            const int r = row0 + rl;
+            if (r >= rows) break;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < PW; ++w) M = fmaxf(M, mg[(w * Sh::ROWS + rl) * MS + HD]);
+            const float ref = softmax_ref(M);
+            tr_f4 o = {0.f, 0.f, 0.f, 0.f};
+            float L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PW; ++w) {
+                const float* e = mg + (w * Sh::ROWS + rl) * MS;
+                const float f = tree_exp2(e[HD] - ref);
+                L = fmaf(f, e[HD + 1], L);
+                o += f * *reinterpret_cast<const tr_f4*>(e + d);
+            }
+            const int nd = r / a.group;
+            put(r, nd, j * a.group + r - nd * a.group, d, o, M, L);
+        }
+    }
+}
+
+// The chunks' partial sums of every row whose context has more than one, in chunk
+// order: grid (ceil(rows n_kv / RB), n_seq), HD / 4 lanes a row.
+template <int HD>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+    constexpr int LPR = HD / 4, RB = 256 / LPR;
+    const int s = blockIdx.y, all_rows = a.max_nodes * a.group;
+    const int len = min(max(a.lens[s], 0), a.max_ctx);
+    const int used = (len + a.chunk - 1) / a.chunk;
+    if (used <= 1) return;
+    const int nodes = a.n_nodes ? min(max(a.n_nodes[s], 0), a.max_nodes) : a.max_nodes;
+    const int x = blockIdx.x * RB + threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
+    const int j = x / all_rows, r = x % all_rows;
+    if (j >= a.n_kv || r >= nodes * a.group) return;
+    const int64_t at = (((int64_t)s * a.n_kv + j) * all_rows + r) * a.nch;
+    float M = -INFINITY;
+    for (int c = 0; c < used; ++c) M = fmaxf(M, a.stats[at + c].x);
+    const float ref = softmax_ref(M);
+    tr_f4 o = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.0f;
+    for (int c = 0; c < used; ++c) {
+        const float2 ml = a.stats[at + c];
+        const float f = tree_exp2(ml.x - ref);
+        L = fmaf(f, ml.y, L);
+        o += f * *reinterpret_cast<const tr_f4*>(a.part + (at + c) * HD + d);
+    }
+    const int nd = r / a.group;
+    float* p = a.out + (int64_t)s * a.ld_out_seq + (int64_t)nd * a.ld_out +
+               (int64_t)(j * a.group + r - nd * a.group) * HD + d;
+    *reinterpret_cast<tr_f4u*>(p) = o / L;
+}
+
 // weights[s, j, t] += sum over the group's heads of 2^(score - m) / l, from the
-// scores and the chunk records' (m, l): grid (ceil(max_ctx / 256), n_kv, n_seq).
+// scores and the chunks' (m, l): grid (ceil(max_ctx / 256), n_kv, n_seq).  unit: what
+// a probability of 1 counts in l.
 __global__ __launch_bounds__(256) void tree_weights_kernel(
-    float* __restrict__ weights, int64_t ld_w, int64_t ld_w_seq, const float* __restrict__ scores,
-    int64_t ld_scores, const float* __restrict__ records, const int32_t* __restrict__ lens,
-    int max_ctx, int n_heads, int group, int hd) {
+    float* __restrict__ weights, int64_t ld_w, int64_t ld_w_seq, TreeArgs a, float unit) {
     const int t = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, s = blockIdx.z;
-    const int len = min(max(lens[s], 0), max_ctx);
+    const int len = min(max(a.lens[s], 0), a.max_ctx);
     if (t >= len) return;
+    const int used = (len + a.chunk - 1) / a.chunk;
     float sum = 0.0f;
-    for (int g = 0; g < group; ++g) {
-        const int64_t h = (int64_t)s * n_heads + (int64_t)j * group + g;
-        const float* rec = records + h * (hd + 2);
-        sum += tree_exp2(scores[h * ld_scores + t] - softmax_ref(rec[hd])) / rec[hd + 1];
+    for (int g = 0; g < a.group; ++g) {
+        const int64_t h = (int64_t)s * a.n_heads + (int64_t)j * a.group + g;
+        float M = -INFINITY, L = 0.0f;
+        for (int c = 0; c < used; ++c) M = fmaxf(M, a.stats[h * a.nch + c].x);
+        const float ref = softmax_ref(M);
+        for (int c = 0; c < used; ++c) {
+            const float2 ml = a.stats[h * a.nch + c];
+            L = fmaf(tree_exp2(ml.x - ref), ml.y, L);
+        }
+        sum += tree_exp2(a.scores[h * a.ld_scores + t] - ref) * unit / L;
     }
     weights[(int64_t)s * ld_w_seq + (int64_t)j * ld_w + t] += sum;
 }
@@ -163,6 +684,85 @@ int tree_any(const TreeArgs& a, int kv_type, int n_seq, hipStream_t stream) {
                : launch(tree_any_kernel<float>, grid, dim3(kWave), 0, stream, a);
 }
 
+// Rows a workgroup takes, by how many a kv head has: no more than there are to 16,
+// 32 or 64, its waves then sharing out the positions; 128 beyond.
+int tree_wg_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+constexpr int kTreeItems = 512;     // workgroups that splits aim for, at most
+constexpr int kTreeChunkMin = 256;  // positions per chunk, at least
+
+// Fewest positions per chunk: their K and V bytes are then several times the
+// chunk's partial sums.
+int tree_chunk_min(int wg_rows) { return wg_rows * 4 > kTreeChunkMin ? wg_rows * 4 : kTreeChunkMin; }
+
+// Rows of partial sums that calls of up to these sizes need: split calls have at
+// most kTreeItems workgroups.
+int64_t tree_part_rows(int n_seq, int max_nodes, int n_heads, int n_heads_kv, int max_ctx) {
+    const int64_t rows = (int64_t)max_nodes * (n_heads / n_heads_kv);
+    const int wr = tree_wg_rows(rows);
+    const int64_t a = (int64_t)kTreeItems * wr;
+    const int64_t b = (int64_t)n_seq * n_heads * max_nodes * ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
+    return a < b ? a : b;
+}
+
+// Splits contexts so that about kTreeItems workgroups share the call; rows of partial
+// sums used.
+int64_t tree_plan(TreeArgs& a, int n_seq, int64_t part_rows) {
+    const int64_t rows = (int64_t)a.max_nodes * a.group;
+    const int wr = tree_wg_rows(rows);
+    const int64_t base = (int64_t)n_seq * a.n_kv * ((rows + wr - 1) / wr);
+    const int cmin = tree_chunk_min(wr);
+    int64_t nch = kTreeItems / base;
+    if (nch > (a.max_ctx + cmin - 1) / cmin) nch = (a.max_ctx + cmin - 1) / cmin;
+    a.chunk = a.max_ctx > 0 ? a.max_ctx : 1;
+    a.nch = 1;
+    if (nch > 1) {
+        const int chunk = (int)((a.max_ctx + nch - 1) / nch + 127) / 128 * 128;
+        const int n = (a.max_ctx + chunk - 1) / chunk;
+        if (n > 1 && (int64_t)n_seq * a.n_heads * a.max_nodes * n <= part_rows) a.chunk = chunk, a.nch = n;
+    }
+    return (int64_t)n_seq * a.n_heads * a.max_nodes * a.nch;
+}
+
+bool tree_fast(const TreeArgs& a, int kv_type) {
+    const int64_t es = kv_type == JINF_HIP_F16 ? 2 : 4;
+    return (a.head_dim == 64 || a.head_dim == 128) && aligned(a.q, 16) && aligned(a.kc, 16) &&
+           aligned(a.vc, 16) && a.ld_q % 4 == 0 && a.ld_q_seq % 4 == 0 && a.ld_pos * es % 16 == 0 &&
+           a.ld_seq * es % 16 == 0 &&
+           a.ld_pos * es <= (1 << 23);  // a tile's positions within 32-bit offsets
+}
+
+template <typename TC, int HD, int R, int RW>
+int tree_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
+    using Sh = TreeShape<TC, HD, R, RW>;
+    const int64_t rows = (int64_t)a.max_nodes * a.group;
+    const int64_t x = (rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv;
+    return launch(tree_mfma_kernel<TC, HD, R, RW>, dim3((unsigned)x, (unsigned)n_seq, (unsigned)a.nch),
+                  dim3(256), Sh::LDS, stream, a);
+}
+
+template <typename TC, int HD>
+int tree_rows_launch(const TreeArgs& a, int n_seq, bool merge, hipStream_t stream) {
+    const int wr = tree_wg_rows((int64_t)a.max_nodes * a.group);
+    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1>(a, n_seq, stream)
+                   : wr == 32 ? tree_launch<TC, HD, 2, 1>(a, n_seq, stream)
+                   : wr == 64 ? tree_launch<TC, HD, 2, 2>(a, n_seq, stream)
+                              : tree_launch<TC, HD, 2, 4>(a, n_seq, stream);
+    if (rc != JINF_HIP_OK || a.nch <= 1 || !merge) return rc;
+    constexpr int RB = 256 / (HD / 4);
+    const int64_t all = (int64_t)a.max_nodes * a.group * a.n_kv;
+    return launch(tree_merge_kernel<HD>, dim3((unsigned)((all + RB - 1) / RB), (unsigned)n_seq), dim3(256), 0,
+                  stream, a);
+}
+
+int tree_mfma(const TreeArgs& a, int kv_type, int n_seq, hipStream_t stream) {
+    if (kv_type == JINF_HIP_F16)
+        return a.head_dim == 64 ? tree_rows_launch<uint16_t, 64>(a, n_seq, true, stream)
+                                : tree_rows_launch<uint16_t, 128>(a, n_seq, true, stream);
+    return a.head_dim == 64 ? tree_rows_launch<float, 64>(a, n_seq, true, stream)
+                            : tree_rows_launch<float, 128>(a, n_seq, true, stream);
+}
+
 }  // namespace
 }  // namespace jinf
 
@@ -170,7 +770,10 @@ extern "C" size_t jinf_attention_tree_workspace_bytes(int n_seq, int max_nodes, 
                                                       int n_heads_kv, int head_dim, int max_ctx) {
     if (n_seq <= 0 || max_nodes <= 0 || n_heads <= 0 || n_heads_kv <= 0 || head_dim <= 0 || max_ctx < 0)
         return 0;
-    return 256;
+    if (n_heads % n_heads_kv != 0 || max_nodes > JINF_HIP_MAX_NODES) return 0;
+    // {m, l} and the sums of each row
+    return (size_t)jinf::tree_part_rows(n_seq, max_nodes, n_heads, n_heads_kv, max_ctx) *
+           (head_dim + 2) * sizeof(float) + 16;
 }
 
 extern "C" int jinf_attention_tree(float* out, int ld_out, int64_t ld_out_seq, const float* q,
@@ -210,14 +813,27 @@ extern "C" int jinf_attention_tree(float* out, int ld_out, int64_t ld_out_seq, c
     a.max_nodes = max_nodes, a.words = (max_nodes + 63) / 64, a.max_ctx = max_ctx;
     a.head_dim = head_dim, a.n_heads = n_heads, a.n_kv = n_heads_kv, a.group = n_heads / n_heads_kv;
     a.c = scale * kLog2e, a.draft_f16 = draft_type == JINF_HIP_F16;
-    (void)workspace_bytes;
-    return tree_any(a, kv_type, n_seq, stream);
+    a.chunk = max_ctx > 0 ? max_ctx : 1, a.nch = 1;
+    if (!tree_fast(a, kv_type)) return tree_any(a, kv_type, n_seq, stream);
+    // workspace: the sums of as many rows as fit, then {m, l}
+    const int64_t fit = workspace && workspace_bytes > 16
+                            ? (int64_t)((workspace_bytes - 16) / ((head_dim + 2) * sizeof(float))) : 0;
+    const int64_t used = tree_plan(a, n_seq, fit);
+    if (a.nch > 1) {
+        a.part = static_cast<float*>(workspace);
+        a.stats = reinterpret_cast<float2*>(a.part + used * head_dim);
+    }
+    return tree_mfma(a, kv_type, n_seq, stream);
 }
 
 extern "C" size_t jinf_attention_scored_workspace_bytes(int n_seq, int n_heads, int n_heads_kv,
                                                         int head_dim, int max_ctx) {
     if (n_seq <= 0 || n_heads <= 0 || n_heads_kv <= 0 || head_dim <= 0 || max_ctx < 0) return 0;
-    return (size_t)n_seq * n_heads * (jinf::scores_ld(max_ctx) + head_dim + 2) * sizeof(float);
+    if (n_heads % n_heads_kv != 0) return 0;
+    // scores, {m, l} of each row's one chunk at least, sums
+    return ((size_t)n_seq * n_heads * (jinf::scores_ld(max_ctx) + 2) +
+            (size_t)jinf::tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx) * (head_dim + 2)) *
+               sizeof(float) + 16;
 }
 
 extern "C" int jinf_attention_decode_scored(float* out, int ld_out, const float* q, int ld_q,
@@ -252,11 +868,15 @@ extern "C" int jinf_attention_decode_scored(float* out, int ld_out, const float*
     a.n_heads = n_heads, a.n_kv = n_heads_kv, a.group = n_heads / n_heads_kv;
     a.c = scale * kLog2e;
     a.scores = static_cast<float*>(workspace), a.ld_scores = scores_ld(max_ctx);
-    a.records = a.scores + (int64_t)n_seq * n_heads * a.ld_scores;
-    rc = tree_any(a, kv_type, n_seq, stream);
+    a.chunk = max_ctx > 0 ? max_ctx : 1, a.nch = 1;
+    a.part = a.scores + (int64_t)n_seq * n_heads * a.ld_scores;
+    const bool fast = tree_fast(a, kv_type);
+    int64_t used = (int64_t)n_seq * n_heads;
+    if (fast) used = tree_plan(a, n_seq, tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx));
+    a.stats = reinterpret_cast<float2*>(a.part + (a.nch > 1 ? used * head_dim : 0));
+    rc = fast ? tree_mfma(a, kv_type, n_seq, stream) : tree_any(a, kv_type, n_seq, stream);
     if (rc != JINF_HIP_OK || max_ctx == 0) return rc;
     return launch(tree_weights_kernel, dim3((unsigned)((max_ctx + 255) / 256), (unsigned)n_heads_kv,
                                             (unsigned)n_seq),
-                  dim3(256), 0, stream, weights, ld_w, ld_w_seq, a.scores, a.ld_scores, a.records,
-                  lens, max_ctx, n_heads, a.group, head_dim);
+                  dim3(256), 0, stream, weights, ld_w, ld_w_seq, a, fast ? 32768.0f : 1.0f);
 }
