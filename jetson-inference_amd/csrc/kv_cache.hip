@@ -55,18 +55,30 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The positions a (sequence, kv head) keeps: grid (n_kv, n_seq).  A radix
-// select over the keys finds the smallest kept one and how many of its equals
-// stay; an ordered pass then writes the kept positions and moves their weights
-// (a weight moves to a lower place or stays, so within the pass a tile is read
-// before it is written, and no later tile's weights are touched).
+// The positions a (sequence, kv head) keeps: grid (n_kv, n_seq), one workgroup each.
+// The weights are read once, NK a thread (segments of 1024 NK where there are more
+// positions).  Three digits of the keys, 11, 11 and 10 bits from the top, each
+// counted in LDS among the keys that share the digits before, give the smallest
+// kept key and how many of its equals stay; a kept position's row is then the
+// number of larger keys before it plus that of equals before it, at most as many as
+// stay, from one count per wave and register.
+//
+// What bounds it: the latency of a few dependent passes in one workgroup, and the
+// LDS additions of the first pass.  (Weights of one magnitude meet in few counters: a
+// wave whose keys all share a digit adds once.)
+// In place a weight moves to a lower row or stays: a segment is in registers before
+// its first row is written, and rows of later segments are not written by it.
+constexpr int kBins = 2048;
+template <int NK>
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
     const float* weights, int64_t ld_w, int64_t ld_w_seq, float* weights_out, int64_t ld_wo,
     int64_t ld_wo_seq, const int32_t* __restrict__ lens, int32_t* __restrict__ list, int fill,
     int budget, int n_first, int n_recent, int max_ctx, int n_kv) {
     constexpr int kWaves = kSelThreads / kWave;
-    __shared__ unsigned hist[256];
-    __shared__ int wsum[2][kWaves];
+    constexpr int kSeg = kSelThreads * NK;
+    __shared__ unsigned hist[kBins];
+    __shared__ unsigned counts[2][NK * kWaves];  // larger, equal: per (register, wave), then sums before
+    __shared__ unsigned wsum[2][kWaves];
     __shared__ unsigned s_digit, s_need;
     const int j = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     const int wave = tid / kWave, lane = tid & (kWave - 1);
@@ -86,106 +98,202 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
     }
     const int lo = n_first, hi = len - n_recent;  // the positions that compete
     unsigned need = (unsigned)(budget - n_first - n_recent);  // of them, how many stay
+    const bool none = need == 0;
+    const int n_seg = (len + kSeg - 1) / kSeg;
+    float wt[NK];
+    auto load = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int t = t0 + i * kSelThreads + tid;
+            wt[i] = t < len ? w[t] : 0.0f;
+        }
+    };
+    load(0);
+    // Sums before each thread of a workgroup's values, and of all of them.
+    auto scan = [&](unsigned v, int which, unsigned& total) {
+        unsigned x = v;
+#pragma unroll
+        for (int o = 1; o < kWave; o *= 2) {
+            const unsigned y = __shfl_up(x, o, kWave);
+            if (lane >= o) x += y;
+        }
+        if (lane == kWave - 1) wsum[which][wave] = x;
+        __syncthreads();
+        unsigned before = 0;
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            if (i < wave) before += wsum[which][i];
+            total += wsum[which][i];
+        }
+        return before + x - v;
+    };
     uint32_t prefix = 0;  // the threshold's digits found so far
-    if (need > 0) {
+    if (!none) {
 #pragma unroll 1
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t digits = pass == 2 ? 1023u : 2047u;
+            const int above = pass == 0 ? 31 : pass == 1 ? 21 : 10;  // shift of the digits before
+            hist[tid] = 0, hist[tid + kSelThreads] = 0;
             __syncthreads();
-            for (int t = lo + tid; t < hi; t += kSelThreads) {
-                const uint32_t k = weight_key(w[t]);
-                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-                    atomicAdd(&hist[(k >> shift) & 255], 1u);
+            for (int seg = 0; seg < n_seg; ++seg) {
+                if (n_seg > 1) load(seg * kSeg);
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const int t = seg * kSeg + i * kSelThreads + tid;
+                    const uint32_t k = weight_key(wt[i]);
+                    const bool in = t >= lo && t < hi && (pass == 0 || (k >> above) == (prefix >> above));
+                    const unsigned long long who = __ballot(in);
+                    if (!who) continue;
+                    const unsigned d = (k >> shift) & digits;
+                    const unsigned d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(who));
+                    if (__ballot(in && d != d0) == 0) {
+                        if (lane == 0) atomicAdd(&hist[d0], (unsigned)__popcll(who));
+                    } else if (in) {
+                        atomicAdd(&hist[d], 1u);
+                    }
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                unsigned left = need;
-                int d = 255;
-                while (hist[d] < left) left -= hist[d--];
-                s_digit = (unsigned)d;
-                s_need = left;
+            // from the largest digit down: the one at which `need` are reached
+            const unsigned h1 = hist[kBins - 1 - 2 * tid], h2 = hist[kBins - 2 - 2 * tid];
+            unsigned total;
+            const unsigned before = scan(h1 + h2, pass & 1, total);
+            if (before < need && need <= before + h1) {
+                s_digit = (unsigned)(kBins - 1 - 2 * tid), s_need = need - before;
+            } else if (before + h1 < need && need <= before + h1 + h2) {
+                s_digit = (unsigned)(kBins - 2 - 2 * tid), s_need = need - before - h1;
             }
             __syncthreads();
             prefix |= s_digit << shift;
             need = s_need;
-            __syncthreads();
         }
     }
-    // need: how many positions whose key equals the threshold stay (0 when
-    // none compete, and then nothing is above the threshold either)
-    const bool none = budget == n_first + n_recent;
-    int n_kept = 0, n_equal = 0;
-    for (int t0 = 0; t0 < len; t0 += kSelThreads) {
-        const int t = t0 + tid;
-        float wt = 0.0f;
-        bool above = false, equal = false;
-        if (t < len) {
-            wt = w[t];
-            if (t < lo || t >= hi) {
-                above = true;
-            } else if (!none) {
-                const uint32_t k = weight_key(wt);
-                above = k > prefix;
-                equal = k == prefix;
+    unsigned n_larger = 0, n_equal = 0;  // in the segments before
+    for (int seg = 0; seg < n_seg; ++seg) {
+        if (n_seg > 1) {
+            __syncthreads();  // (the counts of the segment before have been read)
+            load(seg * kSeg);
+        }
+        auto kind = [&](int i, bool& larger, bool& equal) {
+            const int t = seg * kSeg + i * kSelThreads + tid;
+            const uint32_t k = weight_key(wt[i]);
+            const bool mid = t >= lo && t < hi;
+            larger = t < len && (!mid || (!none && k > prefix));
+            equal = mid && !none && k == prefix;
+        };
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            bool larger, equal;
+            kind(i, larger, equal);
+            const unsigned long long a = __ballot(larger), b = __ballot(equal);
+            if (lane == 0) counts[0][i * kWaves + wave] = __popcll(a), counts[1][i * kWaves + wave] = __popcll(b);
+        }
+        __syncthreads();
+        unsigned total[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned v = tid < NK * kWaves ? counts[x][tid] : 0u;
+            const unsigned before = scan(v, x, total[x]);
+            if (tid < NK * kWaves) counts[x][tid] = before;
+        }
+        __syncthreads();
+        const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            bool larger, equal;
+            kind(i, larger, equal);
+            const unsigned long long a = __ballot(larger), b = __ballot(equal);
+            const unsigned e = n_equal + counts[1][i * kWaves + wave] + __popcll(b & below);
+            if (larger || (equal && e < need)) {
+                const unsigned r = n_larger + counts[0][i * kWaves + wave] + __popcll(a & below) + min(e, need);
+                out[r] = seg * kSeg + i * kSelThreads + tid;
+                wo[r] = wt[i];
             }
         }
-        const unsigned long long below = (1ull << lane) - 1;
-        const unsigned long long eq = __ballot(equal);
-        if (lane == 0) wsum[0][wave] = __popcll(eq);
-        __syncthreads();
-        int before = n_equal + __popcll(eq & below);
-        for (int i = 0; i < kWaves; ++i) {
-            if (i < wave) before += wsum[0][i];
-            n_equal += wsum[0][i];
-        }
-        const bool stays = above || (equal && before < (int)need);
-        const unsigned long long st = __ballot(stays);
-        if (lane == 0) wsum[1][wave] = __popcll(st);
-        __syncthreads();
-        int r = n_kept + __popcll(st & below);
-        for (int i = 0; i < kWaves; ++i) {
-            if (i < wave) r += wsum[1][i];
-            n_kept += wsum[1][i];
-        }
-        if (stays) {
-            out[r] = t;
-            wo[r] = wt;
-        }
-        __syncthreads();
+        n_larger += total[0], n_equal += total[1];
     }
 }
 
-// The kept rows to their places: grid (n_kv, n_seq, 2 planes), rows in order.
-// In place a row moves to a lower position or stays: a step's rows are all
-// read before any is written, and no later step's rows are touched.
+// The kept rows to their places: grid (n_kv slices, n_seq, 2 planes x chunks), rows in
+// order, `w` units of a row a workgroup.  A kept row moves to a lower position or
+// stays.  In place, one workgroup therefore walks all rows of its slice, and a
+// step's rows are all read before its first is written: rows that later steps read
+// lie past them, so the next step's loads are under way meanwhile.  Into other
+// caches, chunks of rows are independent.
+//
+// What bounds it: the rows' bytes, read and written once; with few sequences, how
+// many of them one workgroup keeps in flight (64 KiB here), hence the slices.
+constexpr int kMoveThreads = 1024;
+constexpr int kMoveU = 4;  // units a thread holds per step
+constexpr int kMoveItems = 256;  // workgroups that a call aims for, one a CU
 template <typename U>
-__global__ __launch_bounds__(kKvThreads) void kv_move_kernel(
+__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
     U* ko, U* vo, int64_t ld_pos_out, int64_t ld_seq_out, const U* k, const U* v, int64_t ld_pos,
-    int64_t ld_seq, const int32_t* __restrict__ lens, int32_t* __restrict__ lens_out,
-    const int32_t* __restrict__ list, int budget, int max_ctx, int n_kv, int row_units) {
-    const int j = blockIdx.x, s = blockIdx.y;
+    int64_t ld_seq, const int32_t* lens, int32_t* lens_out, const int32_t* __restrict__ list,
+    int budget, int max_ctx, int n_kv, int row_units, int w, int chunk, int in_place) {
+    const int j = blockIdx.x % n_kv, slice = blockIdx.x / n_kv, s = blockIdx.y;
+    const int plane = blockIdx.z & 1, r_begin = (int)(blockIdx.z >> 1) * chunk;
     const int len = min(max(lens[s], 0), max_ctx);
     const int keep = min(len, budget);
-    const U* src = (blockIdx.z ? v : k) + (int64_t)s * ld_seq + (int64_t)j * row_units;
-    U* dst = (blockIdx.z ? vo : ko) + (int64_t)s * ld_seq_out + (int64_t)j * row_units;
+    // (lens_out may be lens: min(len, budget) is the same number before and after)
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = keep;
+    if (in_place && len <= budget) return;
+    const int r_end = min(keep, r_begin + chunk);
+    const int per = kMoveThreads / w;  // rows side by side
+    const int u = threadIdx.x % w, rl = threadIdx.x / w;
+    const int64_t off = (int64_t)j * row_units + (int64_t)slice * w + u;
+    const U* src = (plane ? v : k) + (int64_t)s * ld_seq + off;
+    U* dst = (plane ? vo : ko) + (int64_t)s * ld_seq_out + off;
     const int32_t* at = list + ((int64_t)s * n_kv + j) * budget;
-    const int64_t total = (int64_t)keep * row_units;
-    for (int64_t i0 = 0; i0 < total; i0 += kKvThreads) {
-        const int64_t i = i0 + threadIdx.x;
-        const int r = (int)(i / row_units), u = (int)(i % row_units);
-        U x{};
-        if (i < total) x = src[(int64_t)at[r] * ld_pos + u];
-        __syncthreads();
-        if (i < total) dst[(int64_t)r * ld_pos_out + u] = x;
-        __syncthreads();
+    const int step = per * kMoveU;
+    int idx[kMoveU];  // the next step's positions
+    U x[kMoveU];
+    auto positions = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < kMoveU; ++i) {
+            const int r = r0 + i * per + rl;
+            idx[i] = rl < per && r < r_end ? at[r] : -1;
+            if (in_place && idx[i] == r) idx[i] = -1;  // stays where it is
+        }
+    };
+    bool moves[kMoveU];
+    auto rows = [&]() {
+#pragma unroll
+        for (int i = 0; i < kMoveU; ++i) {
+            moves[i] = idx[i] >= 0;
+            if (moves[i]) x[i] = src[(int64_t)idx[i] * ld_pos];
+        }
+    };
+    positions(r_begin);
+    rows();
+    for (int r0 = r_begin; r0 < r_end; r0 += step) {
+        U y[kMoveU];
+        bool m[kMoveU];
+        positions(r0 + step);
+#pragma unroll
+        for (int i = 0; i < kMoveU; ++i) y[i] = x[i], m[i] = moves[i];
+        // every thread's rows of this step are in registers before any is written
+        if (in_place) {
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm<0>());
+            __syncthreads();
+        }
+        rows();
+#pragma unroll
+        for (int i = 0; i < kMoveU; ++i)
+            if (m[i]) dst[(int64_t)(r0 + i * per + rl) * ld_pos_out] = y[i];
     }
-    (void)lens_out;
 }
 
-__global__ __launch_bounds__(kKvThreads) void kv_lens_kernel(const int32_t* lens, int32_t* lens_out,
-                                                             int budget, int max_ctx, int n_seq) {
-    const int s = blockIdx.x * kKvThreads + threadIdx.x;
-    if (s < n_seq) lens_out[s] = min(min(max(lens[s], 0), max_ctx), budget);
+// No position stays: lengths of 0, and no kept one.
+__global__ __launch_bounds__(kKvThreads) void kv_none_kernel(int32_t* __restrict__ lens_out, int n_seq,
+                                                             int32_t* __restrict__ kept, int64_t n_kept) {
+    const int64_t stride = (int64_t)gridDim.x * kKvThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kKvThreads + threadIdx.x; i < n_seq || i < n_kept; i += stride) {
+        if (lens_out && i < n_seq) lens_out[i] = 0;
+        if (i < n_kept) kept[i] = -1;
+    }
 }
 
 bool kv_type_ok(int t) { return t == JINF_HIP_F32 || t == JINF_HIP_F16; }
@@ -207,11 +315,33 @@ int kv_move(void* ko, void* vo, int64_t ld_pos_out, int64_t ld_seq_out, const vo
             const void* v, int64_t ld_pos, int64_t ld_seq, const int32_t* lens, int32_t* lens_out,
             const int32_t* list, int budget, int max_ctx, int n_seq, int n_kv, int64_t row_bytes,
             int64_t es, hipStream_t stream) {
-    const int64_t n = (int64_t)sizeof(U) / es;  // elements of a unit (or units of an element: 1)
-    return launch(kv_move_kernel<U>, dim3(n_kv, n_seq, 2), dim3(kKvThreads), 0, stream,
-                  static_cast<U*>(ko), static_cast<U*>(vo), ld_pos_out / n, ld_seq_out / n,
-                  static_cast<const U*>(k), static_cast<const U*>(v), ld_pos / n, ld_seq / n, lens,
-                  lens_out, list, budget, max_ctx, n_kv, (int)(row_bytes / (int64_t)sizeof(U)));
+    const int64_t n = (int64_t)sizeof(U) / es;  // elements of a unit
+    const int row_units = (int)(row_bytes / (int64_t)sizeof(U));
+    const bool in_place = ko == k;
+    const int rows = budget < max_ctx ? budget : max_ctx;
+    // In place with fewer (sequence, kv head, plane) than CUs, rows are cut into
+    // slices of 128, then 64 bytes.
+    int w = row_units;  // (at most 1024)
+    if (in_place && sizeof(U) == 16)
+        for (int cut = 8; cut >= 4; cut /= 2)
+            if (row_units % cut == 0 && cut < w && (int64_t)n_seq * n_kv * 2 * (row_units / w) < kMoveItems) w = cut;
+    // Into other caches: chunks of rows, of one step at least, for about four
+    // workgroups a CU.
+    const int step = kMoveThreads / w * kMoveU;
+    int chunk = rows;
+    if (!in_place) {
+        const int64_t groups = (int64_t)n_seq * n_kv * 2 * (row_units / w);
+        const int64_t nch = groups < 4 * kMoveItems ? 4 * kMoveItems / groups : 1;
+        chunk = (int)(((int64_t)rows + nch - 1) / nch);
+        chunk = (chunk + step - 1) / step * step;
+    }
+    const int64_t chunks = (rows + (int64_t)chunk - 1) / chunk;
+    return launch(kv_move_kernel<U>,
+                  dim3((unsigned)(n_kv * (row_units / w)), (unsigned)n_seq, (unsigned)(2 * chunks)),
+                  dim3(kMoveThreads), 0, stream, static_cast<U*>(ko), static_cast<U*>(vo),
+                  ld_pos_out / n, ld_seq_out / n, static_cast<const U*>(k), static_cast<const U*>(v),
+                  ld_pos / n, ld_seq / n, lens, lens_out, list, budget, max_ctx, n_kv, row_units, w,
+                  chunk, in_place ? 1 : 0);
 }
 
 }  // namespace
@@ -314,28 +444,26 @@ extern "C" int jinf_cache_evict(void* k_out, void* v_out, int64_t ld_pos_out, in
         (!workspace || !aligned(workspace, 16) ||
          workspace_bytes < jinf_cache_evict_workspace_bytes(n_seq, n_heads_kv, budget)))
         return JINF_HIP_ERR_INVALID;
-    if (budget > 0) {
-        int32_t* list = kept ? kept : static_cast<int32_t*>(workspace);
-        int rc = launch(kv_select_kernel, dim3(n_heads_kv, n_seq), dim3(kSelThreads), 0, stream,
-                        weights, ld_w, ld_w_seq, weights_out, ld_wo, ld_wo_seq, lens, list,
-                        kept ? 1 : 0, budget, n_first, n_recent, max_ctx, n_heads_kv);
-        if (rc != JINF_HIP_OK) return rc;
-        // 16-byte units where everything is aligned to them, else single elements
-        const int64_t row = (int64_t)head_dim * es;
-        const bool wide = aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_out, 16) &&
-                          aligned(v_out, 16) && row % 16 == 0 && ld_pos * es % 16 == 0 &&
-                          ld_seq * es % 16 == 0 && ld_pos_out * es % 16 == 0 &&
-                          ld_seq_out * es % 16 == 0;
-#define JINF_KV_MOVE(U)                                                                          \
+    if (rows_out == 0) {  // (no budget, or caches of no positions)
+        if (!lens_out && !kept) return JINF_HIP_OK;
+        return launch(kv_none_kernel, dim3(64), dim3(kKvThreads), 0, stream, lens_out, n_seq, kept,
+                      kept ? (int64_t)n_seq * n_heads_kv * budget : (int64_t)0);
+    }
+    int32_t* list = kept ? kept : static_cast<int32_t*>(workspace);
+    // 4 weights a thread for up to 4096 positions, else 32
+    auto* select = max_ctx <= 4 * kSelThreads ? kv_select_kernel<4> : kv_select_kernel<32>;
+    const int rc = launch(select, dim3(n_heads_kv, n_seq), dim3(kSelThreads), 0, stream, weights, ld_w,
+                          ld_w_seq, weights_out, ld_wo, ld_wo_seq, lens, list, kept ? 1 : 0, budget,
+                          n_first, n_recent, max_ctx, n_heads_kv);
+    if (rc != JINF_HIP_OK) return rc;
+    // 16-byte units where everything is aligned to them, else single elements
+    const int64_t row = (int64_t)head_dim * es;
+    const bool wide = aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_out, 16) &&
+                      aligned(v_out, 16) && row % 16 == 0 && ld_pos * es % 16 == 0 &&
+                      ld_seq * es % 16 == 0 && ld_pos_out * es % 16 == 0 && ld_seq_out * es % 16 == 0;
+#define JINF_KV_MOVE(U)                                                                             \
     kv_move<U>(k_out, v_out, ld_pos_out, ld_seq_out, k_cache, v_cache, ld_pos, ld_seq, lens, lens_out, \
                list, budget, max_ctx, n_seq, n_heads_kv, row, es, stream)
-        if (max_ctx > 0)
-            rc = wide ? JINF_KV_MOVE(u32x4) : es == 2 ? JINF_KV_MOVE(uint16_t) : JINF_KV_MOVE(uint32_t);
+    return wide ? JINF_KV_MOVE(u32x4) : es == 2 ? JINF_KV_MOVE(uint16_t) : JINF_KV_MOVE(uint32_t);
 #undef JINF_KV_MOVE
-        if (rc != JINF_HIP_OK) return rc;
-    }
-    if (lens_out)
-        return launch(kv_lens_kernel, dim3((n_seq + kKvThreads - 1) / kKvThreads), dim3(kKvThreads),
-                      0, stream, lens, lens_out, budget, max_ctx, n_seq);
-    return JINF_HIP_OK;
 }

@@ -12,55 +12,75 @@ it cannot serve.
 import numpy as np
 import torch
 
-from ._lib import lib
-from .ops import JinfError, _act, _check, _ptr, _stream
+from ._lib import F16, F32, JINF_HIP_OK, lib
+from .ops import JinfError
 
 MAX_NODES = 256
 
+# These calls take microseconds on the device, so what is checked on the way is
+# checked with few Python operations.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_TYPES = {torch.float32: F32, torch.float16: F16}
 
-def _here(**tensors):
-    """Every given tensor on the current device."""
+
+def _device(**tensors):
+    """The current device, which holds every given tensor."""
+    if not all(t is None or t.is_cuda for t in tensors.values()):
+        name = next(n for n, t in tensors.items() if t is not None and not t.is_cuda)
+        raise JinfError(f"{name} is not on the HIP device")
+    here = torch.cuda.current_device()
     for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise JinfError(f"{name} is not on the HIP device")
-        if t.device.index != torch.cuda.current_device():
-            raise JinfError(f"{name} is on {t.device}, the current device is "
-                            f"cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != here:
+            raise JinfError(f"{name} is on {t.device}, the current device is cuda:{here}")
+    return here
 
 
 def _ints(name, t, *shape):
-    """A contiguous int32 tensor of this shape (None passes)."""
-    if t is None:
-        return
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    """A contiguous int32 tensor of this shape."""
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise JinfError(f"{name} must be contiguous int32 {list(shape)}")
 
 
 def _floats(name, t, *shape):
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or (t.numel() and t.stride(-1) != 1):
+    """Strides of an fp32 tensor of this shape."""
+    strides = t.stride()
+    if t.dtype is not torch.float32 or t.shape != shape or (strides[-1] != 1 and t.numel()):
         raise JinfError(f"{name} must be fp32 {list(shape)}, contiguous in its last dimension")
+    return strides
 
 
-def _caches(k, v, n_heads_kv, names="k and v caches"):
-    """(n_seq, max_ctx, head_dim) of a pair of caches."""
-    if (k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or
-            (k.numel() and k.stride(2) != 1)):
-        raise JinfError(f"{names} must be two [n_seq, positions, n_heads_kv * head_dim] tensors of "
-                        "one type and layout")
-    if n_heads_kv <= 0 or k.shape[2] % n_heads_kv or k.shape[2] == 0:
+def _caches(k, v, names="k and v caches"):
+    """Shape, strides and type code of a pair of caches or of rows for them."""
+    shape, strides, code = k.shape, k.stride(), _TYPES.get(k.dtype)
+    if (len(shape) != 3 or code is None or v.shape != shape or v.dtype is not k.dtype or
+            v.stride() != strides or (strides[2] != 1 and k.numel())):
+        raise JinfError(f"{names} must be two fp32 or fp16 [n_seq, positions, n_heads_kv * head_dim] "
+                        "tensors of one type and layout")
+    return shape, strides, code
+
+
+def _head_dim(width, n_heads_kv):
+    if n_heads_kv <= 0 or width % n_heads_kv or width == 0:
         raise JinfError("cache width must be n_heads_kv * head_dim")
-    return k.shape[0], k.shape[1], k.shape[2] // n_heads_kv
+    return width // n_heads_kv
 
 
 def _space(workspace, nbytes, device):
     """The caller's workspace, or one of this call's own."""
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        return torch.empty(max(nbytes(), 16), dtype=torch.uint8, device=device)
+    if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise JinfError("workspace must be a contiguous uint8 tensor")
     return workspace
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check(rc, name):
+    if rc != JINF_HIP_OK:
+        raise JinfError(f"{name} returned status {rc}")
 
 
 def tree_mask(parents, device="cuda"):
@@ -101,31 +121,33 @@ def attention_tree(q, k_cache, v_cache, lens, k_draft, v_draft, mask, n_heads, n
     ceil(nodes / 64)]; n_nodes int32 [n_seq]: nodes of each sequence (None: all).
     Rows past them stay as they were in `out` (zeros in a new one).  Returns out
     fp32 like q."""
-    n_seq, max_ctx, hd = _caches(k_cache, v_cache, n_heads_kv)
-    nodes = q.shape[1] if q.dim() == 3 else -1
-    _here(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft, v_draft=v_draft,
-          mask=mask, n_nodes=n_nodes, out=out, workspace=workspace)
-    _floats("q", q, n_seq, nodes, n_heads * hd)
-    dn, dt, _ = _caches(k_draft, v_draft, n_heads_kv, "k and v drafts")
-    if (dn, dt, k_draft.shape[2]) != (n_seq, nodes, k_cache.shape[2]):
+    (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
+    dshape, dst, dt = _caches(k_draft, v_draft, "k and v drafts")
+    hd, nodes = _head_dim(width, n_heads_kv), dshape[1]
+    here = _device(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft,
+                   v_draft=v_draft, mask=mask, n_nodes=n_nodes, out=out, workspace=workspace)
+    if dshape != (n_seq, nodes, width):
         raise JinfError("drafts must be [n_seq, nodes, n_heads_kv * head_dim]")
-    if (mask.dtype != torch.int64 or tuple(mask.shape) != (n_seq, nodes, (nodes + 63) // 64) or
+    qst = _floats("q", q, n_seq, nodes, n_heads * hd)
+    if (mask.dtype is not torch.int64 or mask.shape != (n_seq, nodes, (nodes + 63) // 64) or
             not mask.is_contiguous()):
         raise JinfError("mask must be contiguous int64 [n_seq, nodes, ceil(nodes / 64)]")
     _ints("lens", lens, n_seq)
-    _ints("n_nodes", n_nodes, n_seq)
+    if n_nodes is not None:
+        _ints("n_nodes", n_nodes, n_seq)
     if out is None:
         make = torch.empty if n_nodes is None else torch.zeros
         out = make((n_seq, nodes, n_heads * hd), dtype=torch.float32, device=q.device)
-    _floats("out", out, n_seq, nodes, n_heads * hd)
-    workspace = _space(workspace, lib().jinf_attention_tree_workspace_bytes(
+    ost = _floats("out", out, n_seq, nodes, n_heads * hd)
+    L = lib()
+    workspace = _space(workspace, lambda: L.jinf_attention_tree_workspace_bytes(
         n_seq, nodes, n_heads, n_heads_kv, hd, max_ctx), q.device)
-    _check(lib().jinf_attention_tree(
-        _ptr(out), out.stride(1), out.stride(0), _ptr(q), q.stride(1), q.stride(0), _ptr(k_cache),
-        _ptr(v_cache), _act(k_cache), k_cache.stride(1), k_cache.stride(0), _ptr(lens),
-        _ptr(k_draft), _ptr(v_draft), _act(k_draft), k_draft.stride(1), k_draft.stride(0),
-        _ptr(mask), _ptr(n_nodes), nodes, n_seq, max_ctx, hd, n_heads, n_heads_kv, float(scale),
-        _ptr(workspace), workspace.numel(), _stream()), "jinf_attention_tree")
+    _check(L.jinf_attention_tree(
+        out.data_ptr(), ost[1], ost[0], q.data_ptr(), qst[1], qst[0], k_cache.data_ptr(),
+        v_cache.data_ptr(), kt, kst[1], kst[0], lens.data_ptr(), k_draft.data_ptr(),
+        v_draft.data_ptr(), dt, dst[1], dst[0], mask.data_ptr(), _ptr(n_nodes), nodes, n_seq,
+        max_ctx, hd, n_heads, n_heads_kv, scale, workspace.data_ptr(), workspace.numel(),
+        _raw_stream(here)), "jinf_attention_tree")
     return out
 
 
@@ -136,26 +158,28 @@ def cache_append(k_cache, v_cache, lens, k_rows, v_rows, n_heads_kv, index=None,
     counts[s] (every one: None); rows past the cache's end are dropped, an index
     outside the rows stores zeros.  weights: the new positions' accumulated
     weights are set to 0.  Returns the new lengths (lens_out; not lens itself)."""
-    n_seq, max_ctx, hd = _caches(k_cache, v_cache, n_heads_kv)
-    rn, rows, _ = _caches(k_rows, v_rows, n_heads_kv, "k and v rows")
-    if rn != n_seq or k_rows.shape[2] != k_cache.shape[2]:
-        raise JinfError("rows must be [n_seq, rows, n_heads_kv * head_dim]")
-    take = rows if index is None else index.shape[-1]
+    (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
+    (rn, rows, rwidth), rst, rt = _caches(k_rows, v_rows, "k and v rows")
+    hd = _head_dim(width, n_heads_kv)
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
-    _here(k_cache=k_cache, v_cache=v_cache, lens=lens, k_rows=k_rows, v_rows=v_rows, index=index,
-          counts=counts, weights=weights, lens_out=lens_out)
+    here = _device(k_cache=k_cache, v_cache=v_cache, lens=lens, k_rows=k_rows, v_rows=v_rows,
+                   index=index, counts=counts, weights=weights, lens_out=lens_out)
+    if rn != n_seq or rwidth != width:
+        raise JinfError("rows must be [n_seq, rows, n_heads_kv * head_dim]")
     _ints("lens", lens, n_seq)
     _ints("lens_out", lens_out, n_seq)
-    _ints("index", index, n_seq, take)
-    _ints("counts", counts, n_seq)
-    if weights is not None:
-        _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
+    take = rows
+    if index is not None:
+        take = index.shape[-1]
+        _ints("index", index, n_seq, take)
+    if counts is not None:
+        _ints("counts", counts, n_seq)
+    wst = (0, 0) if weights is None else _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
     _check(lib().jinf_cache_append(
-        _ptr(k_cache), _ptr(v_cache), _act(k_cache), k_cache.stride(1), k_cache.stride(0),
-        _ptr(weights), weights.stride(1) if weights is not None else 0,
-        weights.stride(0) if weights is not None else 0, _ptr(lens), _ptr(lens_out), _ptr(k_rows),
-        _ptr(v_rows), _act(k_rows), k_rows.stride(1), k_rows.stride(0), rows, _ptr(index),
-        _ptr(counts), take, n_seq, max_ctx, hd, n_heads_kv, _stream()), "jinf_cache_append")
+        k_cache.data_ptr(), v_cache.data_ptr(), kt, kst[1], kst[0], _ptr(weights), wst[1], wst[0],
+        lens.data_ptr(), lens_out.data_ptr(), k_rows.data_ptr(), v_rows.data_ptr(), rt, rst[1],
+        rst[0], rows, _ptr(index), _ptr(counts), take, n_seq, max_ctx, hd, n_heads_kv,
+        _raw_stream(here)), "jinf_cache_append")
     return lens_out
 
 
@@ -171,22 +195,24 @@ def attention_decode_scored(q, k_cache, v_cache, lens, weights, n_heads, n_heads
     """attention_decode that also adds each position's attention weight, summed over
     the query heads of a kv head, to weights fp32 [n_seq, n_heads_kv, max_ctx] in
     place.  Returns out fp32 [n_seq, n_heads * hd]."""
-    n_seq, max_ctx, hd = _caches(k_cache, v_cache, n_heads_kv)
-    _here(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, weights=weights, out=out,
-          workspace=workspace)
-    _floats("q", q, n_seq, n_heads * hd)
-    _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
+    (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
+    hd = _head_dim(width, n_heads_kv)
+    here = _device(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, weights=weights, out=out,
+                   workspace=workspace)
+    qst = _floats("q", q, n_seq, n_heads * hd)
+    wst = _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
     _ints("lens", lens, n_seq)
     if out is None:
         out = torch.empty((n_seq, n_heads * hd), dtype=torch.float32, device=q.device)
-    _floats("out", out, n_seq, n_heads * hd)
-    workspace = _space(workspace, lib().jinf_attention_scored_workspace_bytes(
+    ost = _floats("out", out, n_seq, n_heads * hd)
+    L = lib()
+    workspace = _space(workspace, lambda: L.jinf_attention_scored_workspace_bytes(
         n_seq, n_heads, n_heads_kv, hd, max_ctx), q.device)
-    _check(lib().jinf_attention_decode_scored(
-        _ptr(out), out.stride(0), _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache),
-        _act(k_cache), k_cache.stride(1), k_cache.stride(0), _ptr(weights), weights.stride(1),
-        weights.stride(0), _ptr(lens), n_seq, max_ctx, hd, n_heads, n_heads_kv, float(scale),
-        _ptr(workspace), workspace.numel(), _stream()), "jinf_attention_decode_scored")
+    _check(L.jinf_attention_decode_scored(
+        out.data_ptr(), ost[0], q.data_ptr(), qst[0], k_cache.data_ptr(), v_cache.data_ptr(), kt,
+        kst[1], kst[0], weights.data_ptr(), wst[1], wst[0], lens.data_ptr(), n_seq, max_ctx, hd,
+        n_heads, n_heads_kv, scale, workspace.data_ptr(), workspace.numel(), _raw_stream(here)),
+        "jinf_attention_decode_scored")
     return out
 
 
@@ -206,33 +232,35 @@ def cache_evict(k_cache, v_cache, weights, lens, n_heads_kv, budget, n_first=0, 
     with min(budget, max_ctx) positions or more).  kept: int32 [n_seq, n_heads_kv,
     budget] receives the old positions (-1 past the new length).  Returns the new
     lengths min(lens, budget) (lens_out; may be lens)."""
-    n_seq, max_ctx, hd = _caches(k_cache, v_cache, n_heads_kv)
-    given = [t is not None for t in (k_out, v_out, weights_out)]
-    if any(given) != all(given):
+    (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
+    hd = _head_dim(width, n_heads_kv)
+    wst = _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
+    if k_out is None and v_out is None and weights_out is None:
+        k_out, v_out, weights_out, ost, wost = k_cache, v_cache, weights, kst, wst
+    elif k_out is None or v_out is None or weights_out is None:
         raise JinfError("k_out, v_out and weights_out go together")
-    if not any(given):
-        k_out, v_out, weights_out = k_cache, v_cache, weights
-    on, rows, _ = _caches(k_out, v_out, n_heads_kv, "k and v outputs")
-    if (on, k_out.shape[2], k_out.dtype) != (n_seq, k_cache.shape[2], k_cache.dtype):
-        raise JinfError("outputs must have the caches' type, sequences and width")
-    if rows < min(int(budget), max_ctx):
-        raise JinfError("outputs hold fewer positions than stay")
+    else:
+        (on, rows, owidth), ost, ot = _caches(k_out, v_out, "k and v outputs")
+        if on != n_seq or owidth != width or ot != kt:
+            raise JinfError("outputs must have the caches' type, sequences and width")
+        if rows < min(budget, max_ctx):
+            raise JinfError("outputs hold fewer positions than stay")
+        wost = _floats("weights_out", weights_out, n_seq, n_heads_kv, rows)
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
-    _here(k_cache=k_cache, v_cache=v_cache, weights=weights, lens=lens, k_out=k_out, v_out=v_out,
-          weights_out=weights_out, lens_out=lens_out, kept=kept, workspace=workspace)
-    _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
-    _floats("weights_out", weights_out, n_seq, n_heads_kv, rows)
+    here = _device(k_cache=k_cache, v_cache=v_cache, weights=weights, lens=lens, k_out=k_out,
+                   v_out=v_out, weights_out=weights_out, lens_out=lens_out, kept=kept,
+                   workspace=workspace)
     _ints("lens", lens, n_seq)
     _ints("lens_out", lens_out, n_seq)
-    _ints("kept", kept, n_seq, n_heads_kv, int(budget))
-    workspace = _space(workspace, lib().jinf_cache_evict_workspace_bytes(n_seq, n_heads_kv,
-                                                                         int(budget)),
-                       k_cache.device)
-    _check(lib().jinf_cache_evict(
-        _ptr(k_out), _ptr(v_out), k_out.stride(1), k_out.stride(0), _ptr(k_cache), _ptr(v_cache),
-        _act(k_cache), k_cache.stride(1), k_cache.stride(0), _ptr(weights_out),
-        weights_out.stride(1), weights_out.stride(0), _ptr(weights), weights.stride(1),
-        weights.stride(0), _ptr(lens), _ptr(lens_out), _ptr(kept), int(budget), int(n_first),
-        int(n_recent), n_seq, max_ctx, hd, n_heads_kv, _ptr(workspace), workspace.numel(),
-        _stream()), "jinf_cache_evict")
+    if kept is not None:
+        _ints("kept", kept, n_seq, n_heads_kv, budget)
+    L = lib()
+    workspace = _space(workspace, lambda: L.jinf_cache_evict_workspace_bytes(
+        n_seq, n_heads_kv, budget), k_cache.device)
+    _check(L.jinf_cache_evict(
+        k_out.data_ptr(), v_out.data_ptr(), ost[1], ost[0], k_cache.data_ptr(), v_cache.data_ptr(),
+        kt, kst[1], kst[0], weights_out.data_ptr(), wost[1], wost[0], weights.data_ptr(), wst[1],
+        wst[0], lens.data_ptr(), lens_out.data_ptr(), _ptr(kept), budget, n_first, n_recent, n_seq,
+        max_ctx, hd, n_heads_kv, workspace.data_ptr(), workspace.numel(), _raw_stream(here)),
+        "jinf_cache_evict")
     return lens_out
