@@ -47,69 +47,69 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(
             weights[(int64_t)s * ld_w_seq + (int64_t)j * ld_w + t] = 0.0f;
 }
 
-// A weight as an unsigned number of the same order: NaN above everything, -0
-// equal to +0.
+// A weight as an unsigned number of the same order: -0 equal to +0, NaN above every
+// number, and above it the positions that stay whatever their weight; 0 is no key.
+constexpr uint32_t kKeyStays = 0xFFFFFFFFu, kKeyNan = 0xFFFFFFFEu;
 __device__ __forceinline__ uint32_t weight_key(float w) {
-    if (w != w) return 0xFFFFFFFFu;
-    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return w != w ? kKeyNan : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-// The positions a (sequence, kv head) keeps: grid (n_kv, n_seq), one workgroup each.
-// The weights are read once, NK a thread (segments of 1024 NK where there are more
-// positions).  Three digits of the keys, 11, 11 and 10 bits from the top, each
-// counted in LDS among the keys that share the digits before, give the smallest
-// kept key and how many of its equals stay; a kept position's row is then the
-// number of larger keys before it plus that of equals before it, at most as many as
-// stay, from one count per wave and register.
+// The positions a (sequence, kv head) keeps, those of the `budget` largest keys (the
+// lowest first among equal ones), ascending: grid (n_kv, n_seq), one workgroup each.
+// The keys are put into LDS once (for each pass, in segments of kSegMax, where there
+// are more positions).  Three digits, 11, 11 and 10 bits from the top, each counted
+// in LDS among the keys that share the digits before, give the smallest kept key and
+// how many of its equals stay; a kept position's row is then the number of larger keys
+// before it plus that of equals before it, at most as many as stay.
 //
-// What bounds it: the latency of a few dependent passes in one workgroup, and the
-// LDS additions of the first pass.  (Weights of one magnitude meet in few counters: a
-// wave whose keys all share a digit adds once.)
-// In place a weight moves to a lower row or stays: a segment is in registers before
-// its first row is written, and rows of later segments are not written by it.
+// What bounds it: instruction issue in the one workgroup, hence four keys a read and
+// no range checks; and code size, hence the rolled loops (weights in registers with
+// unrolled passes, 50 KB of code, took 35 us at 8192 positions, fetching
+// instructions).  Weights of one magnitude meet in few counters: a wave whose keys
+// all share a digit adds once.
 constexpr int kBins = 2048;
-template <int NK>
+constexpr int kSelStep = 4 * kSelThreads;
+constexpr int kSegMax = 8 * kSelStep;  // positions held at once, 128 KiB
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
-    const float* weights, int64_t ld_w, int64_t ld_w_seq, float* weights_out, int64_t ld_wo,
-    int64_t ld_wo_seq, const int32_t* __restrict__ lens, int32_t* __restrict__ list, int fill,
-    int budget, int n_first, int n_recent, int max_ctx, int n_kv) {
+    const float* __restrict__ weights, int64_t ld_w, int64_t ld_w_seq, const int32_t* __restrict__ lens,
+    int32_t* __restrict__ list, int fill, int budget, int n_first, int n_recent, int max_ctx, int n_kv) {
     constexpr int kWaves = kSelThreads / kWave;
-    constexpr int kSeg = kSelThreads * NK;
+    extern __shared__ __attribute__((aligned(16))) uint32_t keys[];
     __shared__ unsigned hist[kBins];
-    __shared__ unsigned counts[2][NK * kWaves];  // larger, equal: per (register, wave), then sums before
+    __shared__ unsigned counts[2][kSegMax / kSelStep * kWaves];  // larger, equal: per step and wave, then before
     __shared__ unsigned wsum[2][kWaves];
     __shared__ unsigned s_digit, s_need;
     const int j = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     const int wave = tid / kWave, lane = tid & (kWave - 1);
     const int len = min(max(lens[s], 0), max_ctx);
     const float* w = weights + (int64_t)s * ld_w_seq + (int64_t)j * ld_w;
-    float* wo = weights_out + (int64_t)s * ld_wo_seq + (int64_t)j * ld_wo;
     int32_t* out = list + ((int64_t)s * n_kv + j) * budget;
-    const int keep = min(len, budget);
     if (fill)
-        for (int r = keep + tid; r < budget; r += kSelThreads) out[r] = -1;
+        for (int r = min(len, budget) + tid; r < budget; r += kSelThreads) out[r] = -1;
     if (len <= budget) {
-        for (int r = tid; r < len; r += kSelThreads) {
-            out[r] = r;
-            if (wo != w) wo[r] = w[r];
-        }
+        for (int r = tid; r < len; r += kSelThreads) out[r] = r;
         return;
     }
-    const int lo = n_first, hi = len - n_recent;  // the positions that compete
-    unsigned need = (unsigned)(budget - n_first - n_recent);  // of them, how many stay
-    const bool none = need == 0;
-    const int n_seg = (len + kSeg - 1) / kSeg;
-    float wt[NK];
-    auto load = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int t = t0 + i * kSelThreads + tid;
-            wt[i] = t < len ? w[t] : 0.0f;
+    const int n_seg = (len + kSegMax - 1) / kSegMax;
+    // A segment's keys, 0 up to a whole step; steps in it.
+    auto load = [&](int seg) {
+        const int base = seg * kSegMax, n = min(kSegMax, len - base);
+        const int steps = (n + kSelStep - 1) / kSelStep;
+        if (n_seg > 1) __syncthreads();  // (the keys before have been read)
+#pragma unroll 8
+        for (int at = tid; at < steps * kSelStep; at += kSelThreads) {
+            const int t = base + at;
+            uint32_t k = 0;
+            if (at < n) k = t < n_first || t >= len - n_recent ? kKeyStays : weight_key(w[t]);
+            keys[at] = k;
         }
+        __syncthreads();
+        return steps;
     };
-    load(0);
-    // Sums before each thread of a workgroup's values, and of all of them.
+    int steps = load(0);
+    auto key4 = [&](int st) { return *reinterpret_cast<const uint4*>(keys + st * kSelStep + 4 * tid); };
+    // Sum of the threads' values before each thread, and of all.
     auto scan = [&](unsigned v, int which, unsigned& total) {
         unsigned x = v;
 #pragma unroll
@@ -128,97 +128,107 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
         }
         return before + x - v;
     };
-    uint32_t prefix = 0;  // the threshold's digits found so far
-    if (!none) {
+    uint32_t limit = 0;  // the threshold's digits found so far
+    unsigned need = (unsigned)budget;
 #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            const uint32_t digits = pass == 2 ? 1023u : 2047u;
-            const int above = pass == 0 ? 31 : pass == 1 ? 21 : 10;  // shift of the digits before
-            hist[tid] = 0, hist[tid + kSelThreads] = 0;
-            __syncthreads();
-            for (int seg = 0; seg < n_seg; ++seg) {
-                if (n_seg > 1) load(seg * kSeg);
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+        // keys whose digits before are the threshold's lie in [limit, limit + span]
+        const uint32_t span = pass == 0 ? 0xFFFFFFFFu : pass == 1 ? (1u << 21) - 1 : 1023u;
+        hist[tid] = 0, hist[tid + kSelThreads] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int seg = 0; seg < n_seg; ++seg) {
+            if (n_seg > 1) steps = load(seg);
+#pragma unroll 1
+            for (int st = 0; st < steps; ++st) {
+                const uint4 k4 = key4(st);
+                const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+                bool in[4], any = false;
+                uint32_t d[4];
 #pragma unroll
-                for (int i = 0; i < NK; ++i) {
-                    const int t = seg * kSeg + i * kSelThreads + tid;
-                    const uint32_t k = weight_key(wt[i]);
-                    const bool in = t >= lo && t < hi && (pass == 0 || (k >> above) == (prefix >> above));
-                    const unsigned long long who = __ballot(in);
-                    if (!who) continue;
-                    const unsigned d = (k >> shift) & digits;
-                    const unsigned d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(who));
-                    if (__ballot(in && d != d0) == 0) {
-                        if (lane == 0) atomicAdd(&hist[d0], (unsigned)__popcll(who));
-                    } else if (in) {
-                        atomicAdd(&hist[d], 1u);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    in[e] = k[e] != 0 && k[e] - limit <= span;
+                    d[e] = (k[e] >> shift) & digits;
+                    any |= in[e];
                 }
-            }
-            __syncthreads();
-            // from the largest digit down: the one at which `need` are reached
-            const unsigned h1 = hist[kBins - 1 - 2 * tid], h2 = hist[kBins - 2 - 2 * tid];
-            unsigned total;
-            const unsigned before = scan(h1 + h2, pass & 1, total);
-            if (before < need && need <= before + h1) {
-                s_digit = (unsigned)(kBins - 1 - 2 * tid), s_need = need - before;
-            } else if (before + h1 < need && need <= before + h1 + h2) {
-                s_digit = (unsigned)(kBins - 2 - 2 * tid), s_need = need - before - h1;
-            }
-            __syncthreads();
-            prefix |= s_digit << shift;
-            need = s_need;
-        }
-    }
-    unsigned n_larger = 0, n_equal = 0;  // in the segments before
-    for (int seg = 0; seg < n_seg; ++seg) {
-        if (n_seg > 1) {
-            __syncthreads();  // (the counts of the segment before have been read)
-            load(seg * kSeg);
-        }
-        auto kind = [&](int i, bool& larger, bool& equal) {
-            const int t = seg * kSeg + i * kSelThreads + tid;
-            const uint32_t k = weight_key(wt[i]);
-            const bool mid = t >= lo && t < hi;
-            larger = t < len && (!mid || (!none && k > prefix));
-            equal = mid && !none && k == prefix;
-        };
+                if (!__ballot(any)) continue;
+                const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+                if (!__ballot(!(in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 && d[2] == d0 && d[3] == d0))) {
+                    if (lane == 0) atomicAdd(&hist[d0], 4u * kWave);
+                    continue;
+                }
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            bool larger, equal;
-            kind(i, larger, equal);
-            const unsigned long long a = __ballot(larger), b = __ballot(equal);
-            if (lane == 0) counts[0][i * kWaves + wave] = __popcll(a), counts[1][i * kWaves + wave] = __popcll(b);
+                for (int e = 0; e < 4; ++e)
+                    if (in[e]) atomicAdd(&hist[d[e]], 1u);
+            }
+        }
+        __syncthreads();
+        // from the largest digit down: the one at which `need` are reached
+        const unsigned h1 = hist[kBins - 1 - 2 * tid], h2 = hist[kBins - 2 - 2 * tid];
+        unsigned total;
+        const unsigned before = scan(h1 + h2, pass & 1, total);
+        if (before < need && need <= before + h1 + h2) {
+            const bool first = need <= before + h1;
+            s_digit = (unsigned)(kBins - (first ? 1 : 2) - 2 * tid);
+            s_need = need - before - (first ? 0 : h1);
+        }
+        __syncthreads();
+        limit |= s_digit << shift;
+        need = s_need;
+    }
+    // `limit` is the smallest kept key now, and `need` of its equals stay
+    unsigned n_larger = 0, n_equal = 0;  // in the segments before
+#pragma unroll 1
+    for (int seg = 0; seg < n_seg; ++seg) {
+        if (n_seg > 1) steps = load(seg);
+#pragma unroll 1
+        for (int st = 0; st < steps; ++st) {
+            const uint4 k = key4(st);
+            const unsigned larger = __popcll(__ballot(k.x > limit)) + __popcll(__ballot(k.y > limit)) +
+                                    __popcll(__ballot(k.z > limit)) + __popcll(__ballot(k.w > limit));
+            const unsigned equal = __popcll(__ballot(k.x == limit)) + __popcll(__ballot(k.y == limit)) +
+                                   __popcll(__ballot(k.z == limit)) + __popcll(__ballot(k.w == limit));
+            if (lane == 0) counts[0][st * kWaves + wave] = larger, counts[1][st * kWaves + wave] = equal;
         }
         __syncthreads();
         unsigned total[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const unsigned v = tid < NK * kWaves ? counts[x][tid] : 0u;
+            const unsigned v = tid < steps * kWaves ? counts[x][tid] : 0u;
             const unsigned before = scan(v, x, total[x]);
-            if (tid < NK * kWaves) counts[x][tid] = before;
+            if (tid < steps * kWaves) counts[x][tid] = before;
         }
         __syncthreads();
-        const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll 1
+        for (int st = 0; st < steps; ++st) {
+            const uint4 k4 = key4(st);
+            const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+            unsigned a = n_larger + counts[0][st * kWaves + wave];
+            unsigned b = n_equal + counts[1][st * kWaves + wave];
+            // the lanes before, then this lane's own four in turn
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            bool larger, equal;
-            kind(i, larger, equal);
-            const unsigned long long a = __ballot(larger), b = __ballot(equal);
-            const unsigned e = n_equal + counts[1][i * kWaves + wave] + __popcll(b & below);
-            if (larger || (equal && e < need)) {
-                const unsigned r = n_larger + counts[0][i * kWaves + wave] + __popcll(a & below) + min(e, need);
-                out[r] = seg * kSeg + i * kSelThreads + tid;
-                wo[r] = wt[i];
+            for (int e = 0; e < 4; ++e) {
+                const unsigned long long x = __ballot(k[e] > limit), y = __ballot(k[e] == limit);
+                a = __builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, a));
+                b = __builtin_amdgcn_mbcnt_hi((uint32_t)(y >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)y, b));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool larger = k[e] > limit, equal = k[e] == limit;
+                if (larger || (equal && b < need)) out[a + min(b, need)] = seg * kSegMax + st * kSelStep + 4 * tid + e;
+                a += larger;
+                b += equal;
             }
         }
         n_larger += total[0], n_equal += total[1];
     }
 }
 
-// The kept rows to their places: grid (n_kv slices, n_seq, 2 planes x chunks), rows in
-// order, `w` units of a row a workgroup.  A kept row moves to a lower position or
-// stays.  In place, one workgroup therefore walks all rows of its slice, and a
+// The kept rows to their places: grid (n_kv slices, n_seq, 2 planes x chunks + 1), rows in
+// order, `w` units of a row a workgroup; the last of the third index move the weights
+// (by the workgroups of slice 0).  A kept row moves to a lower position or stays.  In place, one workgroup therefore walks all rows of its slice, and a
 // step's rows are all read before its first is written: rows that later steps read
 // lie past them, so the next step's loads are under way meanwhile.  Into other
 // caches, chunks of rows are independent.
@@ -228,25 +238,12 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
 constexpr int kMoveThreads = 1024;
 constexpr int kMoveU = 4;  // units a thread holds per step
 constexpr int kMoveItems = 256;  // workgroups that a call aims for, one a CU
+// Rows r_begin .. r_end of one workgroup's slice: threads of lane-row rl < per take unit
+// u (already in src and dst) of rows rl, rl + per, ...
 template <typename U>
-__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
-    U* ko, U* vo, int64_t ld_pos_out, int64_t ld_seq_out, const U* k, const U* v, int64_t ld_pos,
-    int64_t ld_seq, const int32_t* lens, int32_t* lens_out, const int32_t* __restrict__ list,
-    int budget, int max_ctx, int n_kv, int row_units, int w, int chunk, int in_place) {
-    const int j = blockIdx.x % n_kv, slice = blockIdx.x / n_kv, s = blockIdx.y;
-    const int plane = blockIdx.z & 1, r_begin = (int)(blockIdx.z >> 1) * chunk;
-    const int len = min(max(lens[s], 0), max_ctx);
-    const int keep = min(len, budget);
-    // (lens_out may be lens: min(len, budget) is the same number before and after)
-    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = keep;
-    if (in_place && len <= budget) return;
-    const int r_end = min(keep, r_begin + chunk);
-    const int per = kMoveThreads / w;  // rows side by side
-    const int u = threadIdx.x % w, rl = threadIdx.x / w;
-    const int64_t off = (int64_t)j * row_units + (int64_t)slice * w + u;
-    const U* src = (plane ? v : k) + (int64_t)s * ld_seq + off;
-    U* dst = (plane ? vo : ko) + (int64_t)s * ld_seq_out + off;
-    const int32_t* at = list + ((int64_t)s * n_kv + j) * budget;
+__device__ __forceinline__ void move_rows(U* dst, int64_t ld_dst, const U* src, int64_t ld_src,
+                                          const int32_t* __restrict__ at, int r_begin, int r_end,
+                                          int per, int rl, bool in_place) {
     const int step = per * kMoveU;
     int idx[kMoveU];  // the next step's positions
     U x[kMoveU];
@@ -263,7 +260,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
 #pragma unroll
         for (int i = 0; i < kMoveU; ++i) {
             moves[i] = idx[i] >= 0;
-            if (moves[i]) x[i] = src[(int64_t)idx[i] * ld_pos];
+            if (moves[i]) x[i] = src[(int64_t)idx[i] * ld_src];
         }
     };
     positions(r_begin);
@@ -282,8 +279,38 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
         rows();
 #pragma unroll
         for (int i = 0; i < kMoveU; ++i)
-            if (m[i]) dst[(int64_t)(r0 + i * per + rl) * ld_pos_out] = y[i];
+            if (m[i]) dst[(int64_t)(r0 + i * per + rl) * ld_dst] = y[i];
     }
+}
+
+template <typename U>
+__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
+    U* ko, U* vo, int64_t ld_pos_out, int64_t ld_seq_out, const U* k, const U* v, int64_t ld_pos,
+    int64_t ld_seq, float* weights_out, int64_t ld_wo, int64_t ld_wo_seq, const float* weights,
+    int64_t ld_w, int64_t ld_w_seq, const int32_t* lens, int32_t* lens_out,
+    const int32_t* __restrict__ list, int budget, int max_ctx, int n_kv, int row_units, int w,
+    int chunk, int in_place) {
+    const int j = blockIdx.x % n_kv, slice = blockIdx.x / n_kv, s = blockIdx.y;
+    const bool is_weights = blockIdx.z == gridDim.z - 1;
+    if (is_weights && slice > 0) return;
+    const int len = min(max(lens[s], 0), max_ctx);
+    const int keep = min(len, budget);
+    // (lens_out may be lens: min(len, budget) is the same number before and after)
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = keep;
+    if (in_place && len <= budget) return;
+    const int32_t* at = list + ((int64_t)s * n_kv + j) * budget;
+    if (is_weights) {
+        move_rows(weights_out + (int64_t)s * ld_wo_seq + (int64_t)j * ld_wo, 1,
+                  weights + (int64_t)s * ld_w_seq + (int64_t)j * ld_w, 1, at, 0, keep, kMoveThreads,
+                  (int)threadIdx.x, in_place);
+        return;
+    }
+    const int plane = blockIdx.z & 1, r_begin = (int)(blockIdx.z >> 1) * chunk;
+    const int u = threadIdx.x % w, rl = threadIdx.x / w;
+    const int64_t off = (int64_t)j * row_units + (int64_t)slice * w + u;
+    move_rows((plane ? vo : ko) + (int64_t)s * ld_seq_out + off, ld_pos_out,
+              (plane ? v : k) + (int64_t)s * ld_seq + off, ld_pos, at, r_begin,
+              min(keep, r_begin + chunk), kMoveThreads / w, rl, in_place);
 }
 
 // No position stays: lengths of 0, and no kept one.
@@ -312,9 +339,10 @@ bool kv_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
 
 template <typename U>
 int kv_move(void* ko, void* vo, int64_t ld_pos_out, int64_t ld_seq_out, const void* k,
-            const void* v, int64_t ld_pos, int64_t ld_seq, const int32_t* lens, int32_t* lens_out,
-            const int32_t* list, int budget, int max_ctx, int n_seq, int n_kv, int64_t row_bytes,
-            int64_t es, hipStream_t stream) {
+            const void* v, int64_t ld_pos, int64_t ld_seq, float* weights_out, int64_t ld_wo,
+            int64_t ld_wo_seq, const float* weights, int64_t ld_w, int64_t ld_w_seq,
+            const int32_t* lens, int32_t* lens_out, const int32_t* list, int budget, int max_ctx,
+            int n_seq, int n_kv, int64_t row_bytes, int64_t es, hipStream_t stream) {
     const int64_t n = (int64_t)sizeof(U) / es;  // elements of a unit
     const int row_units = (int)(row_bytes / (int64_t)sizeof(U));
     const bool in_place = ko == k;
@@ -337,11 +365,11 @@ int kv_move(void* ko, void* vo, int64_t ld_pos_out, int64_t ld_seq_out, const vo
     }
     const int64_t chunks = (rows + (int64_t)chunk - 1) / chunk;
     return launch(kv_move_kernel<U>,
-                  dim3((unsigned)(n_kv * (row_units / w)), (unsigned)n_seq, (unsigned)(2 * chunks)),
+                  dim3((unsigned)(n_kv * (row_units / w)), (unsigned)n_seq, (unsigned)(2 * chunks + 1)),
                   dim3(kMoveThreads), 0, stream, static_cast<U*>(ko), static_cast<U*>(vo),
                   ld_pos_out / n, ld_seq_out / n, static_cast<const U*>(k), static_cast<const U*>(v),
-                  ld_pos / n, ld_seq / n, lens, lens_out, list, budget, max_ctx, n_kv, row_units, w,
-                  chunk, in_place ? 1 : 0);
+                  ld_pos / n, ld_seq / n, weights_out, ld_wo, ld_wo_seq, weights, ld_w, ld_w_seq, lens,
+                  lens_out, list, budget, max_ctx, n_kv, row_units, w, chunk, in_place ? 1 : 0);
 }
 
 }  // namespace
@@ -450,11 +478,10 @@ extern "C" int jinf_cache_evict(void* k_out, void* v_out, int64_t ld_pos_out, in
                       kept ? (int64_t)n_seq * n_heads_kv * budget : (int64_t)0);
     }
     int32_t* list = kept ? kept : static_cast<int32_t*>(workspace);
-    // 4 weights a thread for up to 4096 positions, else 32
-    auto* select = max_ctx <= 4 * kSelThreads ? kv_select_kernel<4> : kv_select_kernel<32>;
-    const int rc = launch(select, dim3(n_heads_kv, n_seq), dim3(kSelThreads), 0, stream, weights, ld_w,
-                          ld_w_seq, weights_out, ld_wo, ld_wo_seq, lens, list, kept ? 1 : 0, budget,
-                          n_first, n_recent, max_ctx, n_heads_kv);
+    const int held = max_ctx < kSegMax ? round_up(max_ctx, kSelStep) : kSegMax;
+    const int rc = launch(kv_select_kernel, dim3(n_heads_kv, n_seq), dim3(kSelThreads), held * sizeof(uint32_t),
+                          stream, weights, ld_w, ld_w_seq, lens, list, kept ? 1 : 0, budget, n_first,
+                          n_recent, max_ctx, n_heads_kv);
     if (rc != JINF_HIP_OK) return rc;
     // 16-byte units where everything is aligned to them, else single elements
     const int64_t row = (int64_t)head_dim * es;
@@ -462,8 +489,9 @@ extern "C" int jinf_cache_evict(void* k_out, void* v_out, int64_t ld_pos_out, in
                       aligned(v_out, 16) && row % 16 == 0 && ld_pos * es % 16 == 0 &&
                       ld_seq * es % 16 == 0 && ld_pos_out * es % 16 == 0 && ld_seq_out * es % 16 == 0;
 #define JINF_KV_MOVE(U)                                                                             \
-    kv_move<U>(k_out, v_out, ld_pos_out, ld_seq_out, k_cache, v_cache, ld_pos, ld_seq, lens, lens_out, \
-               list, budget, max_ctx, n_seq, n_heads_kv, row, es, stream)
+    kv_move<U>(k_out, v_out, ld_pos_out, ld_seq_out, k_cache, v_cache, ld_pos, ld_seq,                 \
+               weights_out, ld_wo, ld_wo_seq, weights, ld_w, ld_w_seq, lens, lens_out, list, budget, max_ctx, \
+               n_seq, n_heads_kv, row, es, stream)
     return wide ? JINF_KV_MOVE(u32x4) : es == 2 ? JINF_KV_MOVE(uint16_t) : JINF_KV_MOVE(uint32_t);
 #undef JINF_KV_MOVE
 }
