@@ -65,8 +65,8 @@ extern "C" {
  *     j / 64 for node j (itself included, if it is to be).  Any relation may be
  *     given; bits at or past the sequence's node count are ignored.
  *   - n_nodes: nodes of each sequence (device int32, clamped to [0,
- *     max_nodes]), or NULL: max_nodes.  Rows past it are neither read nor
- *     written.
+ *     max_nodes]), or NULL: max_nodes.  Output rows past it are not written; what
+ *     the other rows past it hold does not matter.
  *   - ld_seq may be 0 (all sequences share one cached prefix).
  *   - scale as in jinf_attention_decode (0: 1 / sqrt(head_dim)).
  * Fast path: head_dim 64 or 128, q, caches and their strides 16-byte aligned;

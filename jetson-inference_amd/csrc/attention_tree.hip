@@ -26,8 +26,8 @@ struct TreeArgs {
     int64_t ld_out, ld_out_seq, ld_q, ld_q_seq, ld_pos, ld_seq, ld_draft, ld_draft_seq;
     int max_nodes, words, max_ctx, head_dim, n_heads, n_kv, group;
     float c;  // scale * log2(e)
-    float* scores;  // null, or the scores [n_seq][n_heads][ld_scores] wanted
-    int64_t ld_scores;
+    float* scores;  // null, or the scores wanted: [n_seq][n_kv][blocks][group][16], 16 positions a block
+    int64_t blocks;
     int draft_f16;
     // Contexts in chunks of `chunk` positions, nch of them at most; chunk 0 also
     // takes the drafted tokens.  Row (s, j, r) chunk c has its partial sums at
@@ -99,7 +99,8 @@ __global__ __launch_bounds__(64) void tree_any_kernel(TreeArgs a) {
         const int64_t at = (int64_t)t * a.ld_pos;
         const float st = step([&](int d) { return tree_get(kb, at + d); },
                               [&](int d) { return tree_get(vb, at + d); });
-        if (a.scores && lane == 0) a.scores[((int64_t)s * a.n_heads + h) * a.ld_scores + t] = st;
+        if (a.scores && lane == 0)
+            a.scores[((((int64_t)s * a.n_kv + j) * a.blocks + (t >> 4)) * a.group + h % a.group) * 16 + (t & 15)] = st;
     }
     if (mask)
         for (int jn = 0; jn < nodes; ++jn) {
@@ -121,10 +122,10 @@ __global__ __launch_bounds__(64) void tree_any_kernel(TreeArgs a) {
 //
 // Per tile of positions, with the rows (node, head) of one kv head as columns:
 //   S^T[t][r]  = sum_d K[t][d] Q'[d][r]       Q' = c q
-//   O^T[d][r] += sum_t V^T[d][t] P'^T[t][r]   P' = 2^15 2^(S - m)
+//   O^T[d][r] += sum_t V^T[d][t] P'^T[t][r]   P' = 2^11 2^(S - m)
 // Both products leave row r in lane r % 16 of every lane group, so the running
 // maximum, the sum and the rescaling of O are one value a lane, and the scores'
-// accumulators are the second product's operand as they stand.  The 2^15 keeps
+// accumulators are the second product's operand as they stand.  The 2^11 keeps
 // the probabilities of an fp16 product in its normal range; the sum l carries it
 // too, so it cancels.
 //   fp16 cache: v_mfma_f32_16x16x32_f16, Q' and P' as fp16 hi + lo in two products
@@ -138,10 +139,18 @@ __global__ __launch_bounds__(64) void tree_any_kernel(TreeArgs a) {
 // and V from LDS once for its 16 R rows.
 typedef _Float16 tr_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 tr_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 tr_h2 __attribute__((ext_vector_type(2)));
+typedef float tr_f2 __attribute__((ext_vector_type(2)));
 typedef float tr_f4 __attribute__((ext_vector_type(4)));
 typedef float tr_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef short tr_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) tr_s4 tr_lds_s4;
+
+// Probabilities count 2^kTreeUnit in O and l.  A reference that lags the maximum by up
+// to kTreeSlack keeps them below 2^15; the least that an fp16 hi + lo pair resolves,
+// 2^-25, is then 2^-36 of the reference's.  (Following every new maximum cost 40
+// vector operations in a quarter of the steps.)
+constexpr float kTreeUnit = 11.0f, kTreeSlack = 4.0f;
 
 __device__ __forceinline__ tr_h8 tr_cat(tr_h4 a, tr_h4 b) {
     return tr_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -158,28 +167,40 @@ __device__ __forceinline__ void tr_split_product(const float (&x)[4], tr_h4& hi,
 }
 // Of exponentials: plain conversions, since an instruction in inline assembly must
 // not read v_exp's result without the wait that the compiler places for its own.
-__device__ __forceinline__ void tr_split_exp(const float (&x)[4], tr_h4& hi, tr_h4& lo) {
+// minus_one is opaque to the compiler, so that the rest is one mixed-precision FMA.
+__device__ __forceinline__ void tr_split_exp(const float (&x)[4], float minus_one, tr_h4& hi, tr_h4& lo) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        hi[i] = (_Float16)x[i];
-        lo[i] = (_Float16)(x[i] - (float)hi[i]);
+    for (int i = 0; i < 4; i += 2) {
+        const tr_h2 h = __builtin_convertvector((tr_f2{x[i], x[i + 1]}), tr_h2);
+        const tr_f2 rest = {fmaf((float)h[0], minus_one, x[i]), fmaf((float)h[1], minus_one, x[i + 1])};
+        const tr_h2 l = __builtin_convertvector(rest, tr_h2);
+        hi[i] = h[0], hi[i + 1] = h[1];
+        lo[i] = l[0], lo[i + 1] = l[1];
     }
 }
 
-template <typename TC, int HD, int R_, int RW_>
+template <typename TC, int HD, int R_, int RW_, bool SCORE = false>
 struct TreeShape {
     static constexpr bool F16 = sizeof(TC) == 2;
     static constexpr int R = R_, RW = RW_, PW = 4 / RW_;
     static constexpr int ROWS = 16 * R * RW;               // rows per workgroup
-    static constexpr int ST = F16 ? (RW == 4 ? 64 : 128) : (RW == 4 ? 32 : 64);  // positions per tile
-    static constexpr int TP = ST / PW;                     // of them, a wave's
     static constexpr int PITCH = HD * (int)sizeof(TC);     // LDS bytes per row
+    // Positions per tile: 32 KiB of K and V, or 16 positions a wave where that is more.
+    static constexpr int FIT = 16384 / PITCH, LEAST = 16 * PW;
+    static constexpr int ST = RW == 4 ? (FIT < 64 ? FIT : 64) : FIT > LEAST ? FIT : LEAST;
+    static constexpr int TP = ST / PW;                     // of them, a wave's
+    static constexpr int SP = TP < 32 ? TP : 32;           // and those of one softmax step
     static constexpr int CH = PITCH / 16;                  // 16-byte pieces per row
     static constexpr int LD = ST * CH / 256;               // loads per lane per tile (K or V)
     static constexpr int BUF = 2 * ST * PITCH;             // K tile, V tile
+    static constexpr int NS = 2;  // tiles in LDS, NS - 1 on their way
     static constexpr int MERGE = PW > 1 ? PW * ROWS * (HD + 4) * 4 : 0;
-    static constexpr int LDS = 2 * BUF > MERGE ? 2 * BUF : MERGE;
-    static constexpr int WGS = 2 * LDS <= 160 * 1024 ? 2 : 1;  // workgroups per CU
+    // A fifth wave that stores the scores, from two tiles' worth behind the tiles.
+    static constexpr bool STORER = SCORE && R == 1 && RW == 1;
+    static constexpr int THREADS = STORER ? 320 : 256;
+    static constexpr int TILES = NS * BUF > MERGE ? NS * BUF : MERGE;
+    static constexpr int LDS = TILES + (STORER ? 2 * ST * ROWS * 4 : 0);
+    static constexpr int WGS = 2 * LDS <= 159 * 1024 ? 2 : 1;  // workgroups per CU
 };
 
 // LDS place of a row's 16-byte piece c.  K: the 16 rows that a fragment read
@@ -196,13 +217,22 @@ __device__ __forceinline__ int tree_v_at(int r, int c) {
 
 // grid (row tiles * n_kv, n_seq, chunks), 256 threads; the kv head is the fastest
 // index, so that row tiles of one head, which read the same K and V, lie n_kv
-// apart (on one XCD for 8 kv heads).
-template <typename TC, int HD, int R, int RW>
-__global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfma_kernel(TreeArgs a) {
-    using Sh = TreeShape<TC, HD, R, RW>;
+// apart (on one XCD for 8 kv heads).  Heads, row tiles and sequences turn with the
+// slower indices: workgroups go to XCDs, and in one of them to its 4 shader engines,
+// by their number in the grid, so that otherwise an XCD reads one head's addresses
+// alone (64 sequences x 8192, loads only: 335 -> 325 us) and the last, partly filled
+// row tile of every sequence falls to the same shader engine (4 tiles: CUs busy 73% of
+// the time).
+// SCORE: one node a sequence, no drafted tokens, and the scores kept.
+template <typename TC, int HD, int R, int RW, bool SCORE>
+__global__ __launch_bounds__((TreeShape<TC, HD, R, RW, SCORE>::THREADS), (TreeShape<TC, HD, R, RW, SCORE>::WGS))
+void tree_mfma_kernel(TreeArgs a) {
+    using Sh = TreeShape<TC, HD, R, RW, SCORE>;
     constexpr bool F16 = Sh::F16;
     constexpr int PW = Sh::PW, ST = Sh::ST, TP = Sh::TP, PITCH = Sh::PITCH, CH = Sh::CH, LD = Sh::LD;
-    constexpr int NBK = TP / 16;   // 16-position blocks of a wave's part of a tile
+    constexpr int NS = Sh::NS;
+    constexpr int SP = Sh::SP;
+    constexpr int NBK = SP / 16;   // 16-position blocks of a softmax step
     constexpr int NB = HD / 16;    // 16-dim blocks of the output
     constexpr int QV = F16 ? HD / 32 : HD / 4;  // q registers: h8 (hi and lo each) or floats
     extern __shared__ __attribute__((aligned(16))) uint8_t tree_lds[];
@@ -211,17 +241,99 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfm
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int col = lane & 15, lg = lane >> 4;
     const int pw = wave / RW, rw = wave % RW;
-    const int j = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv, s = blockIdx.y, cix = blockIdx.z;
+    const int cix = blockIdx.z, s = (blockIdx.y + cix) % gridDim.y;
+    const int tile = (blockIdx.x / a.n_kv + blockIdx.y + cix) % (gridDim.x / a.n_kv);
+    const int j = (blockIdx.x + blockIdx.y + cix) % a.n_kv;
     const int len = min(max(a.lens[s], 0), a.max_ctx);
     const int nodes = a.n_nodes ? min(max(a.n_nodes[s], 0), a.max_nodes) : a.max_nodes;
     const int rows = nodes * a.group, all_rows = a.max_nodes * a.group;
     const int row0 = tile * Sh::ROWS;
+    // The lane's rows and their q.  (q's loads need neither lengths nor node counts,
+    // and are used up before the tiles' loads: a wait for them is a wait for nothing else.)
+    int node[R], head[R];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        const int r = row0 + (rw * R + g) * 16 + col;
+        node[g] = r < all_rows ? r / a.group : 0;
+        head[g] = j * a.group + (r < all_rows ? r - node[g] * a.group : 0);
+    }
+    tr_h8 qh[R][F16 ? QV : 1], ql[R][F16 ? QV : 1];
+    float qf[R][F16 ? 1 : QV];
+#pragma unroll
+    for (int g = 0; g < R; ++g) {
+        const float* qp = a.q + (int64_t)s * a.ld_q_seq + (int64_t)node[g] * a.ld_q + (int64_t)head[g] * HD;
+        if constexpr (F16) {
+            // 32-deep k-step u: lane group lg holds dims HD / 4 lg + 8 u .. + 7, the
+            // 16-byte piece HD / 32 lg + u of the K row
+#pragma unroll
+            for (int u = 0; u < QV; ++u) {
+                tr_h4 hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float4 v = *reinterpret_cast<const float4*>(qp + HD / 4 * lg + 8 * u + 4 * e);
+                    const float x[4] = {v.x * a.c, v.y * a.c, v.z * a.c, v.w * a.c};
+                    tr_split_product(x, hi[e], lo[e]);
+                }
+                qh[g][u] = tr_cat(hi[0], hi[1]);
+                ql[g][u] = tr_cat(lo[0], lo[1]);
+            }
+        } else {
+            // 4-deep k-step 4 u + i: lane group lg holds dim 16 u + 4 lg + i, element i
+            // of the K row's 16-byte piece 4 u + lg
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u) {
+                const float4 v = *reinterpret_cast<const float4*>(qp + 16 * u + 4 * lg);
+                qf[g][4 * u] = v.x * a.c, qf[g][4 * u + 1] = v.y * a.c;
+                qf[g][4 * u + 2] = v.z * a.c, qf[g][4 * u + 3] = v.w * a.c;
+            }
+        }
+    }
+    // (used up here, not further down)
+#pragma unroll
+    for (int g = 0; g < R; ++g)
+#pragma unroll
+        for (int u = 0; u < QV; ++u) {
+            if constexpr (F16) asm volatile("" : "+v"(qh[g][u]), "+v"(ql[g][u]));
+            else asm volatile("" : "+v"(qf[g][u]));
+        }
+
     const int c0 = cix * a.chunk, c1 = min(len, c0 + a.chunk);
     if (row0 >= rows || (cix > 0 && c0 >= len)) return;  // (workgroup-uniform, before any barrier)
+    bool live[R];
+#pragma unroll
+    for (int g = 0; g < R; ++g) live[g] = row0 + (rw * R + g) * 16 + col < rows;
+    const bool idle = row0 + rw * R * 16 >= rows;  // none of the wave's rows is live
     const int used = max(1, (len + a.chunk - 1) / a.chunk);
-    const int drafts = a.mask && cix == 0 ? nodes : 0;
+    const int drafts = !SCORE && cix == 0 ? nodes : 0;
     const int n_dt = (drafts + ST - 1) / ST;
     const int n_it = n_dt + (max(c1 - c0, 0) + ST - 1) / ST;
+
+    // The scores of one kv head's positions p0 .. lie together, block by block.
+    auto scores_at = [&](int p0) {
+        return a.scores + (((int64_t)s * a.n_kv + j) * a.blocks + (p0 >> 4)) * a.group * 16;
+    };
+    if constexpr (Sh::STORER) {
+        // The fifth wave stores each tile's scores one tile later.  (Stored by the waves
+        // that load, a store's answer holds up those of the loads behind it: 64
+        // sequences x 8192 positions 396 us, without stores 322.)
+        if (wave == 4) {
+            auto store = [&](int it) {
+                const int p0 = c0 + it * ST, n = min(ST, c1 - p0);
+                const float* from = reinterpret_cast<const float*>(tree_lds + Sh::TILES) + (it & 1) * ST * Sh::ROWS;
+                float* to = scores_at(p0);
+                for (int x = 4 * lane; x < (n + 15) / 16 * 16 * a.group; x += 4 * kWave)
+                    *reinterpret_cast<tr_f4*>(to + x) = *reinterpret_cast<const tr_f4*>(from + x);
+            };
+            for (int it = 0; it < n_it; ++it) {
+                __syncthreads();
+                if (it > 0) store(it - 1);
+            }
+            __syncthreads();
+            if (n_it > 0) store(n_it - 1);
+            __syncthreads();
+            return;
+        }
+    }
 
     const char* kb = reinterpret_cast<const char*>(static_cast<const TC*>(a.kc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
     const char* vb = reinterpret_cast<const char*>(static_cast<const TC*>(a.vc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
@@ -252,90 +364,73 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfm
     // caller): their probability is 0 in rows that do not see them, their product not.
     constexpr int EL = 16 / (int)sizeof(TC);  // elements per 16-byte piece
     const int64_t dbase = (int64_t)s * a.ld_draft_seq + (int64_t)j * HD;
+    // K pieces, then V pieces: all of a lane's loads are under way before the first is used.
     auto load_draft = [&](int d0, int buf) {
         uint8_t* base = tree_lds + buf * Sh::BUF;
 #pragma unroll 1
-        for (int i = 0; i < 2 * LD; ++i) {
-            const bool is_v = i >= LD;
-            const int slot = tid + 256 * (is_v ? i - LD : i), r = slot / CH, p = slot % CH;
-            const int c = is_v ? tree_v_at<TC>(r, p) : tree_k_at<TC, HD>(r, p);
-            float e[EL] = {};
-            if (d0 + r < drafts) {
-                const int64_t at = dbase + (int64_t)(d0 + r) * a.ld_draft + (int64_t)c * EL;
-                const void* src = is_v ? a.vd : a.kd;
+        for (int is_v = 0; is_v < 2; ++is_v) {
+            const void* src = is_v ? a.vd : a.kd;
+            float e[LD][EL];
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                const int slot = tid + 256 * i, r = slot / CH, p = slot % CH;
+                const int c = is_v ? tree_v_at<TC>(r, p) : tree_k_at<TC, HD>(r, p);
+                const int64_t at = dbase + (int64_t)min(d0 + r, drafts - 1) * a.ld_draft + (int64_t)c * EL;
+                if (a.draft_f16) {
+                    typedef _Float16 row_h __attribute__((ext_vector_type(EL), aligned(2)));
+                    const row_h h = *reinterpret_cast<const row_h*>(static_cast<const uint16_t*>(src) + at);
+#pragma unroll
+                    for (int x = 0; x < EL; ++x) e[i][x] = (float)h[x];
+                } else {
+#pragma unroll
+                    for (int x = 0; x < EL; x += 4) {
+                        const tr_f4u f = *reinterpret_cast<const tr_f4u*>(static_cast<const float*>(src) + at + x);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) e[i][x + y] = f[y];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                const int slot = tid + 256 * i, r = slot / CH;
                 bool bad = false;
 #pragma unroll
                 for (int x = 0; x < EL; ++x) {
-                    const float f = tree_draft<TC>(src, a.draft_f16, at + x);
-                    const bool nf = is_v && !(fabsf(f) < INFINITY);
+                    // as the cache would hold it: its type's range decides what is finite
+                    const float f = F16 ? h2f(f2h(e[i][x])) : e[i][x];
+                    const bool nf = !(fabsf(f) < INFINITY);
                     bad |= nf;
-                    e[x] = nf ? 0.0f : f;
+                    e[i][x] = (is_v && nf) || d0 + r >= drafts ? 0.0f : f;
                 }
-                if (bad) atomicOr(&s_bad[r >> 5], 1u << (r & 31));
+                if (is_v && bad && d0 + r < drafts) atomicOr(&s_bad[r >> 5], 1u << (r & 31));
+                *reinterpret_cast<uint4*>(base + (is_v ? ST * PITCH : 0) + slot * 16) = Act<TC>::pack(e[i]);
             }
-            *reinterpret_cast<uint4*>(base + (is_v ? ST * PITCH : 0) + slot * 16) = Act<TC>::pack(e);
         }
     };
 
-    // The lane's rows, their mask and q
-    int node[R], head[R];
-    bool live[R];
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        const int r = row0 + (rw * R + g) * 16 + col;
-        live[g] = r < rows;
-        node[g] = live[g] ? r / a.group : 0;
-        head[g] = j * a.group + (live[g] ? r - node[g] * a.group : 0);
-    }
-    const bool idle = row0 + rw * R * 16 >= rows;  // none of the wave's rows is live
-
-    if (tid < 4) s_bad[tid] = 0u;
-    // A first tile of drafted tokens is read by ordinary loads; the first cached
-    // tile is on its way to the other buffer before them.
-    const bool ahead = n_dt == 1 && n_it > 1;
+    // Tiles in order: the drafted tokens', then the cached positions'.  NS - 1 tiles
+    // are under way; a tile of drafted tokens is read by ordinary loads, so the first
+    // one is read after the cached tiles behind it have been asked for.
+    auto stage = [&](int it) {
+        if (it < n_dt) load_draft(it * ST, it % NS);
+        else if (it < n_it) load_cached(c0 + (it - n_dt) * ST, it % NS);
+    };
     if (n_dt > 0) {
-        if (ahead) load_cached(c0, 1);
+        if (tid < 4) s_bad[tid] = 0u;
+        if (n_dt == 1)
+            for (int it = 1; it < NS - 1; ++it) stage(it);
         __syncthreads();  // s_bad
         load_draft(0, 0);
-    } else if (n_it > 0) {
-        load_cached(c0, 0);
+    } else {
+        for (int it = 0; it < NS - 1; ++it) stage(it);
     }
-
-    tr_h8 qh[R][F16 ? QV : 1], ql[R][F16 ? QV : 1];
-    float qf[R][F16 ? 1 : QV];
-#pragma unroll
-    for (int g = 0; g < R; ++g) {
-        const float* qp = a.q + (int64_t)s * a.ld_q_seq + (int64_t)node[g] * a.ld_q + (int64_t)head[g] * HD;
-        const float cs = live[g] ? a.c : 0.0f;
-        if constexpr (F16) {
-            // 32-deep k-step u: lane group lg holds dims HD / 4 lg + 8 u .. + 7, the
-            // 16-byte piece HD / 32 lg + u of the K row
-#pragma unroll
-            for (int u = 0; u < QV; ++u) {
-                tr_h4 hi[2], lo[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float4 v = *reinterpret_cast<const float4*>(qp + HD / 4 * lg + 8 * u + 4 * e);
-                    const float x[4] = {v.x * cs, v.y * cs, v.z * cs, v.w * cs};
-                    tr_split_product(x, hi[e], lo[e]);
-                }
-                qh[g][u] = tr_cat(hi[0], hi[1]);
-                ql[g][u] = tr_cat(lo[0], lo[1]);
-            }
-        } else {
-            // 4-deep k-step 4 u + i: lane group lg holds dim 16 u + 4 lg + i, element i
-            // of the K row's 16-byte piece 4 u + lg
-#pragma unroll
-            for (int u = 0; u < HD / 16; ++u) {
-                const float4 v = *reinterpret_cast<const float4*>(qp + 16 * u + 4 * lg);
-                qf[g][4 * u] = v.x * cs, qf[g][4 * u + 1] = v.y * cs;
-                qf[g][4 * u + 2] = v.z * cs, qf[g][4 * u + 3] = v.w * cs;
-            }
-        }
-    }
+    // (more tiles of drafted tokens, one by one as their buffers come free, below)
+    const int ahead = n_dt > 1 ? 1 : NS - 1;  // tiles staged before the loop
 
     float m[R], lsum[R];
     tr_f4 O[R][NB];
+    float minus_one;
+    asm("s_mov_b32 %0, -1.0" : "=s"(minus_one));
 #pragma unroll
     for (int g = 0; g < R; ++g) {
         m[g] = -INFINITY, lsum[g] = 0.0f;
@@ -343,13 +438,19 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfm
         for (int n = 0; n < NB; ++n) O[g][n] = tr_f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    int buf = 0;
+    int staged = ahead;
 #pragma unroll 1
-    for (int it = 0; it < n_it; ++it, buf ^= 1) {
+    for (int it = 0; it < n_it; ++it) {
         const bool draft = it < n_dt;
         const int t0 = draft ? it * ST : c0 + (it - n_dt) * ST;
-        // this tile has landed for every wave, and every wave is done with the other buffer
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm<0>());
+        const int buf = it % NS;
+        // This tile has landed for every wave once at most the loads of the tiles behind
+        // it are outstanding (they return in order), and every wave is done with the
+        // buffer of the tile before it.
+        const int behind = min(staged, n_it) - 1 - it;
+        if (NS > 3 && behind >= 2) __builtin_amdgcn_s_waitcnt(waitcnt_vm<(NS > 3 ? 4 : 0) * LD>());
+        else if (NS > 2 && behind == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm<(NS > 2 ? 2 : 0) * LD>());
+        else __builtin_amdgcn_s_waitcnt(waitcnt_vm<0>());
         __syncthreads();
         unsigned long long bad = 0;
         if (draft) {
@@ -358,159 +459,175 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfm
             if constexpr (TP < 32) bad = (bad >> (b0 & 31)) & ((1ull << TP) - 1);
             __syncthreads();
             if (tid < 4) s_bad[tid] = 0u;
-            if (it + 1 < n_dt) {
-                __syncthreads();
-                load_draft(t0 + ST, buf ^ 1);
-            }
+            if (it + 1 < n_dt) __syncthreads();  // (the next tile sets bits)
         }
-        if (it + 1 >= n_dt && it + 1 < n_it && !(ahead && it == 0))
-            load_cached(c0 + (it + 1 - n_dt) * ST, buf ^ 1);
-        const int p0 = t0 + pw * TP;  // the wave's first position (or drafted token)
-        const int left = (draft ? drafts : c1) - p0;  // live ones from there
-        if (left <= 0 || idle) continue;  // (wave-uniform)
-        const uint8_t* kst = tree_lds + buf * Sh::BUF + pw * TP * PITCH;
-        const uint8_t* vst = kst + ST * PITCH;
-        tr_f4 S[R][NBK];
-#pragma unroll
-        for (int b = 0; b < NBK; ++b) {
-            const int r = 16 * b + col;
-#pragma unroll
-            for (int g = 0; g < R; ++g) S[g][b] = tr_f4{0.f, 0.f, 0.f, 0.f};
+        // with several tiles of drafted tokens the next one is read now (its bits are
+        // looked at before those of the one after it are set), cached tiles NS - 1 ahead
+        for (const int to = it + 1 < n_dt ? it + 2 : it + NS; staged < to; ++staged) stage(staged);
+        const int end = draft ? drafts : c1;
+        if (idle) continue;  // (wave-uniform)
+#pragma unroll 1
+        for (int sub = pw * TP; sub < (pw + 1) * TP; sub += SP) {
+            const int p0 = t0 + sub;    // the step's first position (or drafted token)
+            const int left = end - p0;  // live ones from there
+            if (left <= 0) break;
+            const uint8_t* kst = tree_lds + buf * Sh::BUF + sub * PITCH;
+            const uint8_t* vst = kst + ST * PITCH;
+            tr_f4 S[R][NBK];
             if constexpr (F16) {
 #pragma unroll
-                for (int u = 0; u < QV; ++u) {
-                    const tr_h8 kf = *reinterpret_cast<const tr_h8*>(
-                        kst + r * PITCH + 16 * tree_k_at<TC, HD>(pw * TP + r, QV * lg + u));
+                for (int u = 0; u < QV; ++u)
 #pragma unroll
-                    for (int g = 0; g < R; ++g) {
-                        S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g][u], S[g][b], 0, 0, 0);
-                        S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][u], S[g][b], 0, 0, 0);
+                    for (int b = 0; b < NBK; ++b) {
+                        const int r = 16 * b + col;
+                        const tr_h8 kf = *reinterpret_cast<const tr_h8*>(
+                            kst + r * PITCH + 16 * tree_k_at<TC, HD>(r, QV * lg + u));
+#pragma unroll
+                        for (int g = 0; g < R; ++g) {
+                            S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                kf, qh[g][u], u ? S[g][b] : tr_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                            S[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][u], S[g][b], 0, 0, 0);
+                        }
                     }
-                }
             } else {
 #pragma unroll
-                for (int u = 0; u < HD / 16; ++u) {
-                    const tr_f4 kf = *reinterpret_cast<const tr_f4*>(
-                        kst + r * PITCH + 16 * tree_k_at<TC, HD>(pw * TP + r, 4 * u + lg));
+                for (int b = 0; b < NBK; ++b) {
+                    const int r = 16 * b + col;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int u = 0; u < HD / 16; ++u) {
+                        const tr_f4 kf = *reinterpret_cast<const tr_f4*>(
+                            kst + r * PITCH + 16 * tree_k_at<TC, HD>(r, 4 * u + lg));
 #pragma unroll
-                        for (int g = 0; g < R; ++g)
-                            S[g][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[g][4 * u + i], S[g][b], 0, 0, 0);
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int g = 0; g < R; ++g)
+                                S[g][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    kf[i], qf[g][4 * u + i], u || i ? S[g][b] : tr_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    }
                 }
             }
-        }
-        if (draft) {
-            // bit 16 b + 4 lg + r: the lane's row sees drafted token p0 + 16 b + 4 lg + r
+            if (draft) {
+                // bit 16 b + 4 lg + r: the lane's row sees drafted token p0 + 16 b + 4 lg + r
 #pragma unroll
-            for (int g = 0; g < R; ++g) {
-                unsigned long long bits = 0;
-                if (live[g]) bits = a.mask[((int64_t)s * a.max_nodes + node[g]) * a.words + (p0 >> 6)] >> (p0 & 63);
-                if (left < 64) bits &= (1ull << left) - 1;
-                bits >>= 4 * lg;
-#pragma unroll
-                for (int b = 0; b < NBK; ++b)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!((bits >> (16 * b + r)) & 1)) S[g][b][r] = -INFINITY;
-            }
-        } else {
-            if (left < TP) {
-#pragma unroll
-                for (int g = 0; g < R; ++g)
+                for (int g = 0; g < R; ++g) {
+                    unsigned bits = 0;
+                    if (live[g])
+                        bits = (unsigned)(a.mask[((int64_t)s * a.max_nodes + node[g]) * a.words + (p0 >> 6)] >> (p0 & 63));
+                    if (left < 32) bits &= (1u << left) - 1;
+                    bits >>= 4 * lg;
 #pragma unroll
                     for (int b = 0; b < NBK; ++b)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (16 * b + 4 * lg + r >= left) S[g][b][r] = -INFINITY;
-            }
-            if (a.scores) {
+                            if (!((bits >> (16 * b + r)) & 1)) S[g][b][r] = -INFINITY;
+                }
+            } else {
+                if (left < SP) {
 #pragma unroll
-                for (int g = 0; g < R; ++g) {
-                    float* sc = a.scores + ((int64_t)s * a.n_heads + head[g]) * a.ld_scores + p0 + 4 * lg;
+                    for (int g = 0; g < R; ++g)
 #pragma unroll
-                    for (int b = 0; b < NBK; ++b)
-                        if (live[g] && 16 * b + 4 * lg < left)
-                            *reinterpret_cast<tr_f4*>(sc + 16 * b) = S[g][b];
+                        for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (16 * b + 4 * lg + r >= left) S[g][b][r] = -INFINITY;
+                }
+                if constexpr (SCORE) {
+                    float* to = scores_at(p0);
+                    if constexpr (Sh::STORER)
+                        to = reinterpret_cast<float*>(tree_lds + Sh::TILES) + (it & 1) * ST * Sh::ROWS +
+                             sub * a.group;
+#pragma unroll
+                    for (int g = 0; g < R; ++g)
+#pragma unroll
+                        for (int b = 0; b < NBK; ++b)
+                            if (live[g] && 16 * b < left)
+                                *reinterpret_cast<tr_f4*>(to + (b * a.group + head[g] - j * a.group) * 16 + 4 * lg) = S[g][b];
                 }
             }
-        }
-        tr_h4 ph[R][F16 ? NBK : 1], pl[R][F16 ? NBK : 1];
+            tr_h4 ph[R][F16 ? NBK : 1], pl[R][F16 ? NBK : 1];
 #pragma unroll
-        for (int g = 0; g < R; ++g) {
-            float tmax = S[g][0][0];
+            for (int g = 0; g < R; ++g) {
+                float tmax = S[g][0][0];
 #pragma unroll
-            for (int b = 0; b < NBK; ++b)
+                for (int b = 0; b < NBK; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, S[g][b][r]);
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 16, kWave));
-            tmax = xor32_max(tmax);
-            if (__ballot(tmax > m[g])) {  // some row's maximum grows: its sums scale down
-                const float mn = fmaxf(m[g], tmax);
-                const float corr = tree_exp2(m[g] - softmax_ref(mn));
-                m[g] = mn;
-                lsum[g] *= corr;
+                    for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, S[g][b][r]);
+                // The reference m follows the maximum only when it falls behind by more than
+                // kTreeSlack (probabilities then stay below 2^15): some row's sums scale down.
+                if (__ballot(tmax > m[g] + kTreeSlack)) {
+                    tmax = fmaxf(tmax, __shfl_xor(tmax, 16, kWave));
+                    tmax = xor32_max(tmax);
+                    const float mn = fmaxf(m[g], tmax);
+                    const float corr = tree_exp2(m[g] - softmax_ref(mn));
+                    m[g] = mn;
+                    lsum[g] *= corr;
 #pragma unroll
-                for (int n = 0; n < NB; ++n) O[g][n] *= corr;
-            }
-            const float ref = softmax_ref(m[g]) - 15.0f;
-            float psum = 0.0f;
-#pragma unroll
-            for (int b = 0; b < NBK; ++b) {
-                float x[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[r] = tree_exp2(S[g][b][r] - ref);
-                    psum += x[r];
+                    for (int n = 0; n < NB; ++n) O[g][n] *= corr;
                 }
-                if constexpr (F16) tr_split_exp(x, ph[g][b], pl[g][b]);
-                else S[g][b] = tr_f4{x[0], x[1], x[2], x[3]};
-            }
-            lsum[g] += psum;
-        }
-        if constexpr (F16) {
-            // V^T[16 n + col][16 b + 4 lg + i], i = 0..3, in one transposing read
-            auto vfrag = [&](int b, int n) {
-                const int vr = 16 * b + 4 * lg + (col >> 2);
-                const int p = tree_v_at<TC>(vr, 2 * n + ((col & 3) >> 1));
-                return __builtin_bit_cast(tr_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                     (tr_lds_s4*)(vst + vr * PITCH + 16 * p + 8 * (col & 1))));
-            };
+                const float ref = softmax_ref(m[g]) - kTreeUnit;
+                float psum;
 #pragma unroll
-            for (int bp = 0; bp < NBK / 2; ++bp)
+                for (int b = 0; b < NBK; ++b) {
+                    float x[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = tree_exp2(S[g][b][r] - ref);
+                        psum = b || r ? psum + x[r] : x[r];
+                    }
+                    if constexpr (F16) tr_split_exp(x, minus_one, ph[g][b], pl[g][b]);
+                    else S[g][b] = tr_f4{x[0], x[1], x[2], x[3]};
+                }
+                lsum[g] += psum;
+            }
+            if constexpr (F16) {
+                // V^T[16 n + col][16 b + 4 lg + i], i = 0..3, in one transposing read
+                auto vfrag = [&](int b, int n) {
+                    const int vr = 16 * b + 4 * lg + (col >> 2);
+                    const int p = tree_v_at<TC>(vr, 2 * n + ((col & 3) >> 1));
+                    return __builtin_bit_cast(tr_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         (tr_lds_s4*)(vst + vr * PITCH + 16 * p + 8 * (col & 1))));
+                };
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const tr_h8 v = tr_cat(vfrag(2 * bp, n), vfrag(2 * bp + 1, n));
+                    if constexpr (NBK == 1) {
+                        const tr_h4 v = vfrag(0, n);
 #pragma unroll
-                    for (int g = 0; g < R; ++g) {
-                        O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            v, tr_cat(ph[g][2 * bp], ph[g][2 * bp + 1]), O[g][n], 0, 0, 0);
-                        O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            v, tr_cat(pl[g][2 * bp], pl[g][2 * bp + 1]), O[g][n], 0, 0, 0);
+                        for (int g = 0; g < R; ++g) {
+                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, ph[g][0], O[g][n], 0, 0, 0);
+                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, pl[g][0], O[g][n], 0, 0, 0);
+                        }
+                    } else {
+                        const tr_h8 v = tr_cat(vfrag(0, n), vfrag(1, n));
+#pragma unroll
+                        for (int g = 0; g < R; ++g) {
+                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, tr_cat(ph[g][0], ph[g][1]), O[g][n], 0, 0, 0);
+                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, tr_cat(pl[g][0], pl[g][1]), O[g][n], 0, 0, 0);
+                        }
                     }
                 }
-        } else {
-            // k-step r: lane group lg holds position 16 b + 4 lg + r
+            } else {
+                // k-step r: lane group lg holds position 16 b + 4 lg + r
 #pragma unroll
-            for (int b = 0; b < NBK; ++b)
+                for (int b = 0; b < NBK; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int vr = 16 * b + 4 * lg + r;
+                    for (int r = 0; r < 4; ++r) {
+                        const int vr = 16 * b + 4 * lg + r;
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        const float v = *reinterpret_cast<const float*>(
-                            vst + vr * PITCH + 16 * tree_v_at<TC>(pw * TP + vr, 4 * n + (col >> 2)) + 4 * (col & 3));
+                        for (int n = 0; n < NB; ++n) {
+                            const float v = *reinterpret_cast<const float*>(
+                                vst + vr * PITCH + 16 * tree_v_at<TC>(vr, 4 * n + (col >> 2)) + 4 * (col & 3));
 #pragma unroll
-                        for (int g = 0; g < R; ++g)
-                            O[g][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[g][b][r], O[g][n], 0, 0, 0);
+                            for (int g = 0; g < R; ++g)
+                                O[g][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, S[g][b][r], O[g][n], 0, 0, 0);
+                        }
                     }
-                }
-        }
-        if (bad) {
+            }
             // non-finite V values: NaN in their dims of the rows that see them
+            unsigned step_bad = (unsigned)(bad >> (sub - pw * TP));
+            if constexpr (SP < 32) step_bad &= (1u << SP) - 1;
 #pragma unroll 1
-            for (unsigned long long left_bad = bad; left_bad; left_bad &= left_bad - 1) {
-                const int d = p0 + __builtin_ctzll(left_bad);
+            for (; step_bad; step_bad &= step_bad - 1) {
+                const int d = p0 + __builtin_ctz(step_bad);
                 const int64_t at = dbase + (int64_t)d * a.ld_draft;
 #pragma unroll
                 for (int g = 0; g < R; ++g) {
@@ -526,7 +643,6 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW>::WGS)) void tree_mfm
             }
         }
     }
-
 #pragma unroll
     for (int g = 0; g < R; ++g) {
         lsum[g] += __shfl_xor(lsum[g], 16, kWave);
@@ -631,33 +747,84 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     *reinterpret_cast<tr_f4u*>(p) = o / L;
 }
 
-// weights[s, j, t] += sum over the group's heads of 2^(score - m) / l, from the
-// scores and the chunks' (m, l): grid (ceil(max_ctx / 256), n_kv, n_seq).  unit: what
-// a probability of 1 counts in l.
-__global__ __launch_bounds__(256) void tree_weights_kernel(
-    float* __restrict__ weights, int64_t ld_w, int64_t ld_w_seq, TreeArgs a, float unit) {
-    const int t = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y, s = blockIdx.z;
+// The scored decode's end: weights[s, j, t] += sum over the group's heads of
+// 2^(score - m) / l, from the scores and the chunks' (m, l), and the chunks' partial
+// sums into out where a context has more than one.  grid (ceil(max_ctx / 1024) or 1,
+// n_kv, n_seq); the first workgroup of each (sequence, kv head) joins the outputs.
+// unit: what a probability of 1 counts in l.
+constexpr int kWtHeads = 64;  // heads whose {reference, unit / l} are held at a time
+__global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ weights, int64_t ld_w,
+                                                          int64_t ld_w_seq, TreeArgs a, float unit) {
+    __shared__ float2 ml[kWtHeads];
+    const int tid = threadIdx.x, j = blockIdx.y, s = blockIdx.z;
     const int len = min(max(a.lens[s], 0), a.max_ctx);
-    if (t >= len) return;
+    const int t0 = blockIdx.x * 1024;
+    if (t0 >= len) return;
     const int used = (len + a.chunk - 1) / a.chunk;
-    float sum = 0.0f;
-    for (int g = 0; g < a.group; ++g) {
-        const int64_t h = (int64_t)s * a.n_heads + (int64_t)j * a.group + g;
-        float M = -INFINITY, L = 0.0f;
-        for (int c = 0; c < used; ++c) M = fmaxf(M, a.stats[h * a.nch + c].x);
-        const float ref = softmax_ref(M);
-        for (int c = 0; c < used; ++c) {
-            const float2 ml = a.stats[h * a.nch + c];
-            L = fmaf(tree_exp2(ml.x - ref), ml.y, L);
+    const int64_t h0 = (int64_t)s * a.n_heads + (int64_t)j * a.group;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const int t = t0 + 4 * tid;
+    for (int g0 = 0; g0 < a.group; g0 += kWtHeads) {
+        const int n = min(kWtHeads, a.group - g0);
+        // 4 lanes a head share its chunks (in the order of the lanes)
+        const int g = tid >> 2, q4 = tid & 3;
+        if (g < n) {
+            const float2* st = a.stats + (h0 + g0 + g) * a.nch;
+            float M = -INFINITY, L = 0.0f;
+            for (int c = q4; c < used; c += 4) M = fmaxf(M, st[c].x);
+            M = fmaxf(M, dpp_f32<0xB1>(M));
+            M = fmaxf(M, dpp_f32<0x4E>(M));
+            const float ref = softmax_ref(M);
+            for (int c = q4; c < used; c += 4) L = fmaf(tree_exp2(st[c].x - ref), st[c].y, L);
+            L += dpp_f32<0xB1>(L);
+            L += dpp_f32<0x4E>(L);
+            if (q4 == 0) ml[g] = make_float2(ref, unit / L);
         }
-        sum += tree_exp2(a.scores[h * a.ld_scores + t] - ref) * unit / L;
+        __syncthreads();
+        if (t < len) {
+            const float* sc = a.scores + ((((int64_t)s * a.n_kv + j) * a.blocks + (t >> 4)) * a.group + g0) * 16 + (t & 15);
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const tr_f4 x = *reinterpret_cast<const tr_f4*>(sc + 16 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = fmaf(tree_exp2(x[e] - ml[i].x), ml[i].y, sum[e]);
+            }
+        }
+        __syncthreads();
     }
-    weights[(int64_t)s * ld_w_seq + (int64_t)j * ld_w + t] += sum;
+    float* w = weights + (int64_t)s * ld_w_seq + (int64_t)j * ld_w + t;
+    if (t + 4 <= len) {
+        *reinterpret_cast<tr_f4u*>(w) = *reinterpret_cast<const tr_f4u*>(w) + tr_f4{sum[0], sum[1], sum[2], sum[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (t + e < len) w[e] += sum[e];
+    }
+    if (blockIdx.x > 0 || used <= 1) return;
+    const int hd = a.head_dim;
+    for (int x = 4 * tid; x < a.group * hd; x += 1024) {
+        const int g = x / hd, d = x % hd;
+        const float2* st = a.stats + (h0 + g) * a.nch;
+        float M = -INFINITY;
+        for (int c = 0; c < used; ++c) M = fmaxf(M, st[c].x);
+        const float ref = softmax_ref(M);
+        const float* part = a.part + (h0 + g) * a.nch * hd + d;
+        tr_f4 o = {0.f, 0.f, 0.f, 0.f};
+        float L = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < used; ++c) {
+            const float f = tree_exp2(st[c].x - ref);
+            L = fmaf(f, st[c].y, L);
+            o += f * *reinterpret_cast<const tr_f4*>(part + (int64_t)c * hd);
+        }
+        *reinterpret_cast<tr_f4u*>(a.out + (int64_t)s * a.ld_out_seq + ((int64_t)j * a.group + g) * hd + d) = o / L;
+    }
 }
 
 constexpr float kLog2e = 1.44269502162933349609375f;
 
-int64_t scores_ld(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
+// 16-position blocks that hold a context's scores
+int64_t score_blocks(int max_ctx) { return ((int64_t)max_ctx + 15) / 16; }
 
 // Shared checks of the caches and the query; n_seq > 0.
 int tree_check(const void* out, const float* q, const void* k, const void* v, int kv_type,
@@ -732,35 +899,37 @@ bool tree_fast(const TreeArgs& a, int kv_type) {
            a.ld_pos * es <= (1 << 23);  // a tile's positions within 32-bit offsets
 }
 
-template <typename TC, int HD, int R, int RW>
+template <typename TC, int HD, int R, int RW, bool SCORE>
 int tree_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
-    using Sh = TreeShape<TC, HD, R, RW>;
+    using Sh = TreeShape<TC, HD, R, RW, SCORE>;
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int64_t x = (rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv;
-    return launch(tree_mfma_kernel<TC, HD, R, RW>, dim3((unsigned)x, (unsigned)n_seq, (unsigned)a.nch),
-                  dim3(256), Sh::LDS, stream, a);
+    return launch(tree_mfma_kernel<TC, HD, R, RW, SCORE>, dim3((unsigned)x, (unsigned)n_seq, (unsigned)a.nch),
+                  dim3(Sh::THREADS), Sh::LDS, stream, a);
 }
 
-template <typename TC, int HD>
-int tree_rows_launch(const TreeArgs& a, int n_seq, bool merge, hipStream_t stream) {
+// SCORE: the scored decode, which joins the chunks' partial sums itself.
+template <typename TC, int HD, bool SCORE>
+int tree_rows_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
     const int wr = tree_wg_rows((int64_t)a.max_nodes * a.group);
-    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1>(a, n_seq, stream)
-                   : wr == 32 ? tree_launch<TC, HD, 2, 1>(a, n_seq, stream)
-                   : wr == 64 ? tree_launch<TC, HD, 2, 2>(a, n_seq, stream)
-                              : tree_launch<TC, HD, 2, 4>(a, n_seq, stream);
-    if (rc != JINF_HIP_OK || a.nch <= 1 || !merge) return rc;
+    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1, SCORE>(a, n_seq, stream)
+                   : wr == 32 ? tree_launch<TC, HD, 2, 1, SCORE>(a, n_seq, stream)
+                   : wr == 64 ? tree_launch<TC, HD, 2, 2, SCORE>(a, n_seq, stream)
+                              : tree_launch<TC, HD, 2, 4, SCORE>(a, n_seq, stream);
+    if (rc != JINF_HIP_OK || a.nch <= 1 || SCORE) return rc;
     constexpr int RB = 256 / (HD / 4);
     const int64_t all = (int64_t)a.max_nodes * a.group * a.n_kv;
     return launch(tree_merge_kernel<HD>, dim3((unsigned)((all + RB - 1) / RB), (unsigned)n_seq), dim3(256), 0,
                   stream, a);
 }
 
+template <bool SCORE>
 int tree_mfma(const TreeArgs& a, int kv_type, int n_seq, hipStream_t stream) {
     if (kv_type == JINF_HIP_F16)
-        return a.head_dim == 64 ? tree_rows_launch<uint16_t, 64>(a, n_seq, true, stream)
-                                : tree_rows_launch<uint16_t, 128>(a, n_seq, true, stream);
-    return a.head_dim == 64 ? tree_rows_launch<float, 64>(a, n_seq, true, stream)
-                            : tree_rows_launch<float, 128>(a, n_seq, true, stream);
+        return a.head_dim == 64 ? tree_rows_launch<uint16_t, 64, SCORE>(a, n_seq, stream)
+                                : tree_rows_launch<uint16_t, 128, SCORE>(a, n_seq, stream);
+    return a.head_dim == 64 ? tree_rows_launch<float, 64, SCORE>(a, n_seq, stream)
+                            : tree_rows_launch<float, 128, SCORE>(a, n_seq, stream);
 }
 
 }  // namespace
@@ -823,7 +992,7 @@ extern "C" int jinf_attention_tree(float* out, int ld_out, int64_t ld_out_seq, c
         a.part = static_cast<float*>(workspace);
         a.stats = reinterpret_cast<float2*>(a.part + used * head_dim);
     }
-    return tree_mfma(a, kv_type, n_seq, stream);
+    return tree_mfma<false>(a, kv_type, n_seq, stream);
 }
 
 extern "C" size_t jinf_attention_scored_workspace_bytes(int n_seq, int n_heads, int n_heads_kv,
@@ -831,7 +1000,7 @@ extern "C" size_t jinf_attention_scored_workspace_bytes(int n_seq, int n_heads, 
     if (n_seq <= 0 || n_heads <= 0 || n_heads_kv <= 0 || head_dim <= 0 || max_ctx < 0) return 0;
     if (n_heads % n_heads_kv != 0) return 0;
     // scores, {m, l} of each row's one chunk at least, sums
-    return ((size_t)n_seq * n_heads * (jinf::scores_ld(max_ctx) + 2) +
+    return ((size_t)n_seq * n_heads * (16 * jinf::score_blocks(max_ctx) + 2) +
             (size_t)jinf::tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx) * (head_dim + 2)) *
                sizeof(float) + 16;
 }
@@ -867,16 +1036,16 @@ extern "C" int jinf_attention_decode_scored(float* out, int ld_out, const float*
     a.max_nodes = 1, a.max_ctx = max_ctx, a.head_dim = head_dim;
     a.n_heads = n_heads, a.n_kv = n_heads_kv, a.group = n_heads / n_heads_kv;
     a.c = scale * kLog2e;
-    a.scores = static_cast<float*>(workspace), a.ld_scores = scores_ld(max_ctx);
+    a.scores = static_cast<float*>(workspace), a.blocks = score_blocks(max_ctx);
     a.chunk = max_ctx > 0 ? max_ctx : 1, a.nch = 1;
-    a.part = a.scores + (int64_t)n_seq * n_heads * a.ld_scores;
+    a.part = a.scores + (int64_t)n_seq * n_heads * a.blocks * 16;
     const bool fast = tree_fast(a, kv_type);
     int64_t used = (int64_t)n_seq * n_heads;
     if (fast) used = tree_plan(a, n_seq, tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx));
     a.stats = reinterpret_cast<float2*>(a.part + (a.nch > 1 ? used * head_dim : 0));
-    rc = fast ? tree_mfma(a, kv_type, n_seq, stream) : tree_any(a, kv_type, n_seq, stream);
+    rc = fast ? tree_mfma<true>(a, kv_type, n_seq, stream) : tree_any(a, kv_type, n_seq, stream);
     if (rc != JINF_HIP_OK || max_ctx == 0) return rc;
-    return launch(tree_weights_kernel, dim3((unsigned)((max_ctx + 255) / 256), (unsigned)n_heads_kv,
-                                            (unsigned)n_seq),
-                  dim3(256), 0, stream, weights, ld_w, ld_w_seq, a, fast ? 32768.0f : 1.0f);
+    return launch(tree_finish_kernel, dim3((unsigned)((max_ctx + 1023) / 1024), (unsigned)n_heads_kv,
+                                           (unsigned)n_seq),
+                  dim3(256), 0, stream, weights, ld_w, ld_w_seq, a, fast ? exp2f(kTreeUnit) : 1.0f);
 }
