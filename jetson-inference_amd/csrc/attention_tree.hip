@@ -179,7 +179,7 @@ __device__ __forceinline__ void tr_split_exp(const float (&x)[4], float minus_on
     }
 }
 
-template <typename TC, int HD, int R_, int RW_, bool SCORE = false>
+template <typename TC, int HD, int R_, int RW_, bool SCORE, bool ONCE>
 struct TreeShape {
     static constexpr bool F16 = sizeof(TC) == 2;
     static constexpr int R = R_, RW = RW_, PW = 4 / RW_;
@@ -193,7 +193,10 @@ struct TreeShape {
     static constexpr int CH = PITCH / 16;                  // 16-byte pieces per row
     static constexpr int LD = ST * CH / 256;               // loads per lane per tile (K or V)
     static constexpr int BUF = 2 * ST * PITCH;             // K tile, V tile
-    static constexpr int NS = 2;  // tiles in LDS, NS - 1 on their way
+    // Tiles in LDS, NS - 1 of them on their way.  Two workgroups a CU with two tiles each,
+    // but one with four where few rows stream caches of many megabytes (64 sequences x
+    // 8192 with scores: 353 against 389 us; 6 fp32 sequences x 3001: 29.6 against 19.5).
+    static constexpr int NS = ONCE && RW == 1 && BUF <= 32768 ? 4 : 2;
     static constexpr int MERGE = PW > 1 ? PW * ROWS * (HD + 4) * 4 : 0;
     // A fifth wave that stores the scores, from two tiles' worth behind the tiles.
     static constexpr bool STORER = SCORE && R == 1 && RW == 1;
@@ -224,10 +227,12 @@ __device__ __forceinline__ int tree_v_at(int r, int c) {
 // row tile of every sequence falls to the same shader engine (4 tiles: CUs busy 73% of
 // the time).
 // SCORE: one node a sequence, no drafted tokens, and the scores kept.
-template <typename TC, int HD, int R, int RW, bool SCORE>
-__global__ __launch_bounds__((TreeShape<TC, HD, R, RW, SCORE>::THREADS), (TreeShape<TC, HD, R, RW, SCORE>::WGS))
+// ONCE: the caches are read once and are larger than what the Infinity Cache keeps.
+template <typename TC, int HD, int R, int RW, bool SCORE, bool ONCE>
+__global__ __launch_bounds__((TreeShape<TC, HD, R, RW, SCORE, ONCE>::THREADS),
+                             (TreeShape<TC, HD, R, RW, SCORE, ONCE>::WGS))
 void tree_mfma_kernel(TreeArgs a) {
-    using Sh = TreeShape<TC, HD, R, RW, SCORE>;
+    using Sh = TreeShape<TC, HD, R, RW, SCORE, ONCE>;
     constexpr bool F16 = Sh::F16;
     constexpr int PW = Sh::PW, ST = Sh::ST, TP = Sh::TP, PITCH = Sh::PITCH, CH = Sh::CH, LD = Sh::LD;
     constexpr int NS = Sh::NS;
@@ -354,6 +359,13 @@ void tree_mfma_kernel(TreeArgs a) {
         const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<char*>(vb + at), (short)0, nrec, 0x00020000);
         uint8_t* base = tree_lds + buf * Sh::BUF + 1024 * wave;
+        if constexpr (ONCE) {
+#pragma unroll
+            for (int i = 0; i < LD; ++i) lds_load16_buf_nt(krs, koff[i], 0, base + 4096 * i);
+#pragma unroll
+            for (int i = 0; i < LD; ++i) lds_load16_buf_nt(vrs, voff[i], 0, base + ST * PITCH + 4096 * i);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < LD; ++i) lds_load16_buf(krs, koff[i], 0, base + 4096 * i);
 #pragma unroll
@@ -749,8 +761,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 
 // The scored decode's end: weights[s, j, t] += sum over the group's heads of
 // 2^(score - m) / l, from the scores and the chunks' (m, l), and the chunks' partial
-// sums into out where a context has more than one.  grid (ceil(max_ctx / 1024) or 1,
-// n_kv, n_seq); the first workgroup of each (sequence, kv head) joins the outputs.
+// sums into out where a context has more than one.  grid (ceil(max_ctx / 1024), and one
+// more where contexts are split, n_kv, n_seq); that last workgroup of each (sequence,
+// kv head) joins the outputs.
 // unit: what a probability of 1 counts in l.
 constexpr int kWtHeads = 64;  // heads whose {reference, unit / l} are held at a time
 __global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ weights, int64_t ld_w,
@@ -759,9 +772,32 @@ __global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ we
     const int tid = threadIdx.x, j = blockIdx.y, s = blockIdx.z;
     const int len = min(max(a.lens[s], 0), a.max_ctx);
     const int t0 = blockIdx.x * 1024;
-    if (t0 >= len) return;
     const int used = (len + a.chunk - 1) / a.chunk;
     const int64_t h0 = (int64_t)s * a.n_heads + (int64_t)j * a.group;
+    if (a.nch > 1 && blockIdx.x == gridDim.x - 1) {
+        if (used <= 1) return;
+        const int hd = a.head_dim;
+        for (int x = 4 * tid; x < a.group * hd; x += 1024) {
+            const int g = x / hd, d = x % hd;
+            const float2* st = a.stats + (h0 + g) * a.nch;
+            float M = -INFINITY;
+#pragma unroll 4
+            for (int c = 0; c < used; ++c) M = fmaxf(M, st[c].x);
+            const float ref = softmax_ref(M);
+            const float* part = a.part + (h0 + g) * a.nch * hd + d;
+            tr_f4 o = {0.f, 0.f, 0.f, 0.f};
+            float L = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < used; ++c) {
+                const float f = tree_exp2(st[c].x - ref);
+                L = fmaf(f, st[c].y, L);
+                o += f * *reinterpret_cast<const tr_f4*>(part + (int64_t)c * hd);
+            }
+            *reinterpret_cast<tr_f4u*>(a.out + (int64_t)s * a.ld_out_seq + ((int64_t)j * a.group + g) * hd + d) = o / L;
+        }
+        return;
+    }
+    if (t0 >= len) return;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     const int t = t0 + 4 * tid;
     for (int g0 = 0; g0 < a.group; g0 += kWtHeads) {
@@ -800,25 +836,6 @@ __global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ we
         for (int e = 0; e < 4; ++e)
             if (t + e < len) w[e] += sum[e];
     }
-    if (blockIdx.x > 0 || used <= 1) return;
-    const int hd = a.head_dim;
-    for (int x = 4 * tid; x < a.group * hd; x += 1024) {
-        const int g = x / hd, d = x % hd;
-        const float2* st = a.stats + (h0 + g) * a.nch;
-        float M = -INFINITY;
-        for (int c = 0; c < used; ++c) M = fmaxf(M, st[c].x);
-        const float ref = softmax_ref(M);
-        const float* part = a.part + (h0 + g) * a.nch * hd + d;
-        tr_f4 o = {0.f, 0.f, 0.f, 0.f};
-        float L = 0.0f;
-#pragma unroll 4
-        for (int c = 0; c < used; ++c) {
-            const float f = tree_exp2(st[c].x - ref);
-            L = fmaf(f, st[c].y, L);
-            o += f * *reinterpret_cast<const tr_f4*>(part + (int64_t)c * hd);
-        }
-        *reinterpret_cast<tr_f4u*>(a.out + (int64_t)s * a.ld_out_seq + ((int64_t)j * a.group + g) * hd + d) = o / L;
-    }
 }
 
 constexpr float kLog2e = 1.44269502162933349609375f;
@@ -856,35 +873,56 @@ int tree_any(const TreeArgs& a, int kv_type, int n_seq, hipStream_t stream) {
 int tree_wg_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr int kTreeItems = 512;     // workgroups that splits aim for, at most
-constexpr int kTreeChunkMin = 256;  // positions per chunk, at least
+constexpr int kTreeChunkMin = 128;  // positions per chunk, at least
 
-// Fewest positions per chunk: their K and V bytes are then several times the
-// chunk's partial sums.
-int tree_chunk_min(int wg_rows) { return wg_rows * 4 > kTreeChunkMin ? wg_rows * 4 : kTreeChunkMin; }
+// Fewest positions per chunk: twice a workgroup's rows, so that the K and V bytes of
+// an fp16 chunk are at least twice those of its partial sums.  (4 times: 5 sequences
+// x 13 nodes x 1999 fp32 positions 32.2 against 29.9 us.  256 positions at least: 7
+// nodes x 333 positions 17.5 against 15.6 us.)
+int tree_chunk_min(int wg_rows) { return wg_rows * 2 > kTreeChunkMin ? wg_rows * 2 : kTreeChunkMin; }
 
 // Rows of partial sums that calls of up to these sizes need: split calls have at
-// most kTreeItems workgroups.
+// most tree_items workgroups.
 int64_t tree_part_rows(int n_seq, int max_nodes, int n_heads, int n_heads_kv, int max_ctx) {
     const int64_t rows = (int64_t)max_nodes * (n_heads / n_heads_kv);
     const int wr = tree_wg_rows(rows);
-    const int64_t a = (int64_t)kTreeItems * wr;
+    const int64_t a = (int64_t)kTreeItems * (wr <= 32 ? 4 : 1) * wr;
     const int64_t b = (int64_t)n_seq * n_heads * max_nodes * ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
     return a < b ? a : b;
 }
 
+// Caches that hold more than this are not expected in the Infinity Cache (256 MB) when
+// they are read again; where no two workgroups read the same rows either, K and V are
+// loaded past it, which leaves it to the scores and partial sums (64 sequences x 8192
+// positions with scores 396 -> 367 us).
+constexpr int64_t kTreeOnceBytes = (int64_t)128 << 20;
+bool tree_once(const TreeArgs& a, int kv_type, int n_seq) {
+    const int64_t es = kv_type == JINF_HIP_F16 ? 2 : 4;
+    return (int64_t)a.max_nodes * a.group <= 128 && a.ld_seq != 0 &&
+           (int64_t)n_seq * a.max_ctx * a.n_kv * a.head_dim * es * 2 > kTreeOnceBytes;
+}
+
+// Workgroups to aim for: what the chip holds at once (more add their own starts and
+// ends: 16 x 25 x 4096 70 us at 512, 78 at 1024), but four times as many where few
+// rows stream large caches, whose ragged ends then even out (64 x 8192 with scores, 389
+// us at 2048, 418 at 512).
+int64_t tree_items(const TreeArgs& a, int kv_type, int n_seq) {
+    return (int64_t)a.max_nodes * a.group <= 32 && tree_once(a, kv_type, n_seq) ? 4 * kTreeItems : kTreeItems;
+}
+
 // Splits contexts so that about kTreeItems workgroups share the call; rows of partial
 // sums used.
-int64_t tree_plan(TreeArgs& a, int n_seq, int64_t part_rows) {
+int64_t tree_plan(TreeArgs& a, int kv_type, int n_seq, int64_t part_rows) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int wr = tree_wg_rows(rows);
     const int64_t base = (int64_t)n_seq * a.n_kv * ((rows + wr - 1) / wr);
     const int cmin = tree_chunk_min(wr);
-    int64_t nch = kTreeItems / base;
+    int64_t nch = tree_items(a, kv_type, n_seq) / base;
     if (nch > (a.max_ctx + cmin - 1) / cmin) nch = (a.max_ctx + cmin - 1) / cmin;
     a.chunk = a.max_ctx > 0 ? a.max_ctx : 1;
     a.nch = 1;
     if (nch > 1) {
-        const int chunk = (int)((a.max_ctx + nch - 1) / nch + 127) / 128 * 128;
+        const int chunk = (int)((a.max_ctx + nch - 1) / nch + 63) / 64 * 64;
         const int n = (a.max_ctx + chunk - 1) / chunk;
         if (n > 1 && (int64_t)n_seq * a.n_heads * a.max_nodes * n <= part_rows) a.chunk = chunk, a.nch = n;
     }
@@ -900,22 +938,23 @@ bool tree_fast(const TreeArgs& a, int kv_type) {
 }
 
 template <typename TC, int HD, int R, int RW, bool SCORE>
-int tree_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
-    using Sh = TreeShape<TC, HD, R, RW, SCORE>;
+int tree_launch(const TreeArgs& a, int n_seq, bool once, hipStream_t stream) {
+    using Sh = TreeShape<TC, HD, R, RW, SCORE, false>;
+    using Big = TreeShape<TC, HD, R, RW, SCORE, true>;
     const int64_t rows = (int64_t)a.max_nodes * a.group;
-    const int64_t x = (rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv;
-    return launch(tree_mfma_kernel<TC, HD, R, RW, SCORE>, dim3((unsigned)x, (unsigned)n_seq, (unsigned)a.nch),
-                  dim3(Sh::THREADS), Sh::LDS, stream, a);
+    const dim3 grid((unsigned)((rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv), (unsigned)n_seq, (unsigned)a.nch);
+    return once ? launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, true>, grid, dim3(Big::THREADS), Big::LDS, stream, a)
+                : launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, false>, grid, dim3(Sh::THREADS), Sh::LDS, stream, a);
 }
 
 // SCORE: the scored decode, which joins the chunks' partial sums itself.
 template <typename TC, int HD, bool SCORE>
-int tree_rows_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
+int tree_rows_launch(const TreeArgs& a, int n_seq, bool once, hipStream_t stream) {
     const int wr = tree_wg_rows((int64_t)a.max_nodes * a.group);
-    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1, SCORE>(a, n_seq, stream)
-                   : wr == 32 ? tree_launch<TC, HD, 2, 1, SCORE>(a, n_seq, stream)
-                   : wr == 64 ? tree_launch<TC, HD, 2, 2, SCORE>(a, n_seq, stream)
-                              : tree_launch<TC, HD, 2, 4, SCORE>(a, n_seq, stream);
+    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1, SCORE>(a, n_seq, once, stream)
+                   : wr == 32 ? tree_launch<TC, HD, 2, 1, SCORE>(a, n_seq, once, stream)
+                   : wr == 64 ? tree_launch<TC, HD, 2, 2, SCORE>(a, n_seq, once, stream)
+                              : tree_launch<TC, HD, 2, 4, SCORE>(a, n_seq, once, stream);
     if (rc != JINF_HIP_OK || a.nch <= 1 || SCORE) return rc;
     constexpr int RB = 256 / (HD / 4);
     const int64_t all = (int64_t)a.max_nodes * a.group * a.n_kv;
@@ -925,11 +964,12 @@ int tree_rows_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
 
 template <bool SCORE>
 int tree_mfma(const TreeArgs& a, int kv_type, int n_seq, hipStream_t stream) {
+    const bool once = tree_once(a, kv_type, n_seq);
     if (kv_type == JINF_HIP_F16)
-        return a.head_dim == 64 ? tree_rows_launch<uint16_t, 64, SCORE>(a, n_seq, stream)
-                                : tree_rows_launch<uint16_t, 128, SCORE>(a, n_seq, stream);
-    return a.head_dim == 64 ? tree_rows_launch<float, 64, SCORE>(a, n_seq, stream)
-                            : tree_rows_launch<float, 128, SCORE>(a, n_seq, stream);
+        return a.head_dim == 64 ? tree_rows_launch<uint16_t, 64, SCORE>(a, n_seq, once, stream)
+                                : tree_rows_launch<uint16_t, 128, SCORE>(a, n_seq, once, stream);
+    return a.head_dim == 64 ? tree_rows_launch<float, 64, SCORE>(a, n_seq, once, stream)
+                            : tree_rows_launch<float, 128, SCORE>(a, n_seq, once, stream);
 }
 
 }  // namespace
@@ -987,7 +1027,7 @@ extern "C" int jinf_attention_tree(float* out, int ld_out, int64_t ld_out_seq, c
     // workspace: the sums of as many rows as fit, then {m, l}
     const int64_t fit = workspace && workspace_bytes > 16
                             ? (int64_t)((workspace_bytes - 16) / ((head_dim + 2) * sizeof(float))) : 0;
-    const int64_t used = tree_plan(a, n_seq, fit);
+    const int64_t used = tree_plan(a, kv_type, n_seq, fit);
     if (a.nch > 1) {
         a.part = static_cast<float*>(workspace);
         a.stats = reinterpret_cast<float2*>(a.part + used * head_dim);
@@ -1041,11 +1081,11 @@ extern "C" int jinf_attention_decode_scored(float* out, int ld_out, const float*
     a.part = a.scores + (int64_t)n_seq * n_heads * a.blocks * 16;
     const bool fast = tree_fast(a, kv_type);
     int64_t used = (int64_t)n_seq * n_heads;
-    if (fast) used = tree_plan(a, n_seq, tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx));
+    if (fast) used = tree_plan(a, kv_type, n_seq, tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx));
     a.stats = reinterpret_cast<float2*>(a.part + (a.nch > 1 ? used * head_dim : 0));
     rc = fast ? tree_mfma<true>(a, kv_type, n_seq, stream) : tree_any(a, kv_type, n_seq, stream);
     if (rc != JINF_HIP_OK || max_ctx == 0) return rc;
-    return launch(tree_finish_kernel, dim3((unsigned)((max_ctx + 1023) / 1024), (unsigned)n_heads_kv,
+    return launch(tree_finish_kernel, dim3((unsigned)((max_ctx + 1023) / 1024 + (a.nch > 1 ? 1 : 0)), (unsigned)n_heads_kv,
                                            (unsigned)n_seq),
                   dim3(256), 0, stream, weights, ld_w, ld_w_seq, a, fast ? exp2f(kTreeUnit) : 1.0f);
 }

@@ -23,15 +23,16 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _TYPES = {torch.float32: F32, torch.float16: F16}
 
 
-def _device(**tensors):
-    """The current device, which holds every given tensor."""
-    if not all(t is None or t.is_cuda for t in tensors.values()):
-        name = next(n for n, t in tensors.items() if t is not None and not t.is_cuda)
-        raise JinfError(f"{name} is not on the HIP device")
-    here = torch.cuda.current_device()
-    for name, t in tensors.items():
+def _device(names, *tensors):
+    """The current device, which holds every given tensor (names: theirs, for the error)."""
+    here = torch.cuda.current_device() if torch.cuda.is_initialized() else -2
+    for i, t in enumerate(tensors):
         if t is not None and t.get_device() != here:
-            raise JinfError(f"{name} is on {t.device}, the current device is cuda:{here}")
+            name = names.split()[i]
+            if not t.is_cuda:
+                raise JinfError(f"{name} is not on the HIP device")
+            raise JinfError(f"{name} is on {t.device}, the current device is "
+                            f"cuda:{torch.cuda.current_device()}")
     return here
 
 
@@ -124,8 +125,8 @@ def attention_tree(q, k_cache, v_cache, lens, k_draft, v_draft, mask, n_heads, n
     (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
     dshape, dst, dt = _caches(k_draft, v_draft, "k and v drafts")
     hd, nodes = _head_dim(width, n_heads_kv), dshape[1]
-    here = _device(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, k_draft=k_draft,
-                   v_draft=v_draft, mask=mask, n_nodes=n_nodes, out=out, workspace=workspace)
+    here = _device("q k_cache v_cache lens k_draft v_draft mask n_nodes out workspace", q, k_cache,
+                   v_cache, lens, k_draft, v_draft, mask, n_nodes, out, workspace)
     if dshape != (n_seq, nodes, width):
         raise JinfError("drafts must be [n_seq, nodes, n_heads_kv * head_dim]")
     qst = _floats("q", q, n_seq, nodes, n_heads * hd)
@@ -162,8 +163,8 @@ def cache_append(k_cache, v_cache, lens, k_rows, v_rows, n_heads_kv, index=None,
     (rn, rows, rwidth), rst, rt = _caches(k_rows, v_rows, "k and v rows")
     hd = _head_dim(width, n_heads_kv)
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
-    here = _device(k_cache=k_cache, v_cache=v_cache, lens=lens, k_rows=k_rows, v_rows=v_rows,
-                   index=index, counts=counts, weights=weights, lens_out=lens_out)
+    here = _device("k_cache v_cache lens k_rows v_rows index counts weights lens_out", k_cache,
+                   v_cache, lens, k_rows, v_rows, index, counts, weights, lens_out)
     if rn != n_seq or rwidth != width:
         raise JinfError("rows must be [n_seq, rows, n_heads_kv * head_dim]")
     _ints("lens", lens, n_seq)
@@ -197,8 +198,8 @@ def attention_decode_scored(q, k_cache, v_cache, lens, weights, n_heads, n_heads
     place.  Returns out fp32 [n_seq, n_heads * hd]."""
     (n_seq, max_ctx, width), kst, kt = _caches(k_cache, v_cache)
     hd = _head_dim(width, n_heads_kv)
-    here = _device(q=q, k_cache=k_cache, v_cache=v_cache, lens=lens, weights=weights, out=out,
-                   workspace=workspace)
+    here = _device("q k_cache v_cache lens weights out workspace", q, k_cache, v_cache, lens,
+                   weights, out, workspace)
     qst = _floats("q", q, n_seq, n_heads * hd)
     wst = _floats("weights", weights, n_seq, n_heads_kv, max_ctx)
     _ints("lens", lens, n_seq)
@@ -247,9 +248,9 @@ def cache_evict(k_cache, v_cache, weights, lens, n_heads_kv, budget, n_first=0, 
             raise JinfError("outputs hold fewer positions than stay")
         wost = _floats("weights_out", weights_out, n_seq, n_heads_kv, rows)
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
-    here = _device(k_cache=k_cache, v_cache=v_cache, weights=weights, lens=lens, k_out=k_out,
-                   v_out=v_out, weights_out=weights_out, lens_out=lens_out, kept=kept,
-                   workspace=workspace)
+    here = _device("k_cache v_cache weights lens k_out v_out weights_out lens_out kept workspace",
+                   k_cache, v_cache, weights, lens, k_out, v_out, weights_out, lens_out, kept,
+                   workspace)
     _ints("lens", lens, n_seq)
     _ints("lens_out", lens_out, n_seq)
     if kept is not None:
