@@ -20,31 +20,42 @@ __device__ __forceinline__ TC as_cached(TR v) {
     else return h2f(v);
 }
 
-// grid (n_take, n_seq), one appended row a workgroup.
-template <typename TC, typename TR>
+// Appended rows, V elements of K or V a thread: grid (ceil(n_take 2 kvw / V / 256), n_seq).
+// What bounds it: the rows' bytes, read and written once (64 sequences x 76 rows of
+// 1024 fp32 to fp16 on average: 17.4 us one element a thread at a time, 12.6 here).
+template <typename TC, typename TR, int V>
 __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(
     TC* __restrict__ kc, TC* __restrict__ vc, int64_t ld_pos, int64_t ld_seq,
     float* __restrict__ weights, int64_t ld_w, int64_t ld_w_seq, const int32_t* __restrict__ lens,
     int32_t* __restrict__ lens_out, const TR* __restrict__ kr, const TR* __restrict__ vr,
     int64_t ld_rows, int64_t ld_rows_seq, int n_rows, const int32_t* __restrict__ index,
-    const int32_t* __restrict__ counts, int n_take, int max_ctx, int kvw, int n_kv) {
-    const int a = blockIdx.x, s = blockIdx.y;
+    const int32_t* __restrict__ counts, int n_take, int max_ctx, int units, int n_kv) {
+    typedef TC VC __attribute__((ext_vector_type(V), aligned(V == 8 ? 16 : sizeof(TC))));
+    typedef TR VR __attribute__((ext_vector_type(V), aligned(V == 8 ? 16 : sizeof(TR))));
+    const int s = blockIdx.y;
     const int len = min(max(lens[s], 0), max_ctx);
     const int count = counts ? min(max(counts[s], 0), n_take) : n_take;
-    if (a == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = min(len + count, max_ctx);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = min(len + count, max_ctx);
+    const int64_t x = (int64_t)blockIdx.x * kKvThreads + threadIdx.x;
+    const int a = (int)(x / (2 * units)), u = (int)(x - (int64_t)a * 2 * units);
     const int t = len + a;
     if (a >= count || t >= max_ctx) return;
+    const bool is_v = u >= units;
+    const int e = (is_v ? u - units : u) * V;
     const int row = index ? index[(int64_t)s * n_take + a] : a;
-    const bool live = row >= 0 && row < n_rows;
-    const int64_t src = (int64_t)s * ld_rows_seq + (int64_t)(live ? row : 0) * ld_rows;
-    const int64_t dst = (int64_t)s * ld_seq + (int64_t)t * ld_pos;
-    for (int e = threadIdx.x; e < kvw; e += kKvThreads) {
-        kc[dst + e] = live ? as_cached<TC, TR>(kr[src + e]) : TC(0);
-        vc[dst + e] = live ? as_cached<TC, TR>(vr[src + e]) : TC(0);
+    VC o = {};
+    if (row >= 0 && row < n_rows) {
+        const VR r = *reinterpret_cast<const VR*>((is_v ? vr : kr) + (int64_t)s * ld_rows_seq + (int64_t)row * ld_rows + e);
+        if constexpr (sizeof(TC) == sizeof(TR)) {
+            o = r;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = as_cached<TC, TR>(r[i]);
+        }
     }
-    if (weights)
-        for (int j = threadIdx.x; j < n_kv; j += kKvThreads)
-            weights[(int64_t)s * ld_w_seq + (int64_t)j * ld_w + t] = 0.0f;
+    *reinterpret_cast<VC*>((is_v ? vc : kc) + (int64_t)s * ld_seq + (int64_t)t * ld_pos + e) = o;
+    if (weights && !is_v)
+        for (int j = u; j < n_kv; j += units) weights[(int64_t)s * ld_w_seq + (int64_t)j * ld_w + t] = 0.0f;
 }
 
 // A weight as an unsigned number of the same order: -0 equal to +0, NaN above every
@@ -64,11 +75,13 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // before it plus that of equals before it, at most as many as stay.
 //
 // What bounds it: instruction issue in the one workgroup, hence four keys a read and
-// no range checks; and code size, hence the rolled loops (weights in registers with
+// no range checks, and few keys left for the last digit; and code size, hence the rolled loops (weights in registers with
 // unrolled passes, 50 KB of code, took 35 us at 8192 positions, fetching
 // instructions).  Weights of one magnitude meet in few counters: a wave whose keys
 // all share a digit adds once.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kBins = 2048;
+constexpr int kSelFew = 2048;  // keys that share the threshold's first digits, gathered if no more
 constexpr int kSelStep = 4 * kSelThreads;
 constexpr int kSegMax = 8 * kSelStep;  // positions held at once, 128 KiB
 __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
@@ -79,7 +92,8 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
     __shared__ unsigned hist[kBins];
     __shared__ unsigned counts[2][kSegMax / kSelStep * kWaves];  // larger, equal: per step and wave, then before
     __shared__ unsigned wsum[2][kWaves];
-    __shared__ unsigned s_digit, s_need;
+    __shared__ uint32_t few[kSelFew];
+    __shared__ unsigned s_digit, s_need, s_here, s_few;
     const int j = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     const int wave = tid / kWave, lane = tid & (kWave - 1);
     const int len = min(max(lens[s], 0), max_ctx);
@@ -98,11 +112,22 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
         const int steps = (n + kSelStep - 1) / kSelStep;
         if (n_seg > 1) __syncthreads();  // (the keys before have been read)
 #pragma unroll 8
-        for (int at = tid; at < steps * kSelStep; at += kSelThreads) {
-            const int t = base + at;
-            uint32_t k = 0;
-            if (at < n) k = t < n_first || t >= len - n_recent ? kKeyStays : weight_key(w[t]);
-            keys[at] = k;
+        for (int st = 0; st < steps; ++st) {
+            const int at = st * kSelStep + 4 * tid, t = base + at;
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (at + 4 <= n) {
+                const f32x4u v = *reinterpret_cast<const f32x4u*>(w + t);
+                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < n) x[e] = w[t + e];
+            }
+            uint32_t k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                k[e] = at + e >= n ? 0u : t + e < n_first || t + e >= len - n_recent ? kKeyStays : weight_key(x[e]);
+            *reinterpret_cast<uint4*>(keys + at) = make_uint4(k[0], k[1], k[2], k[3]);
         }
         __syncthreads();
         return steps;
@@ -130,6 +155,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
     };
     uint32_t limit = 0;  // the threshold's digits found so far
     unsigned need = (unsigned)budget;
+    unsigned here = 0, n_few = 0;  // keys that share the threshold's first digit, and those in `few`
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
@@ -137,31 +163,46 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
         // keys whose digits before are the threshold's lie in [limit, limit + span]
         const uint32_t span = pass == 0 ? 0xFFFFFFFFu : pass == 1 ? (1u << 21) - 1 : 1023u;
         hist[tid] = 0, hist[tid + kSelThreads] = 0;
+        if (pass == 0 && tid == 0) s_few = 0;
         __syncthreads();
+        const bool gather = pass == 1 && here <= kSelFew;  // this pass reads every key, the next these
+        if (pass == 2 && here <= kSelFew && n_few > 0) {
+            for (unsigned i = tid; i < n_few; i += kSelThreads) {
+                const uint32_t k = few[i];
+                if (k - limit <= span) atomicAdd(&hist[(k >> shift) & digits], 1u);
+            }
+        } else {
 #pragma unroll 1
-        for (int seg = 0; seg < n_seg; ++seg) {
-            if (n_seg > 1) steps = load(seg);
+            for (int seg = 0; seg < n_seg; ++seg) {
+                if (n_seg > 1) steps = load(seg);
 #pragma unroll 1
-            for (int st = 0; st < steps; ++st) {
-                const uint4 k4 = key4(st);
-                const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-                bool in[4], any = false;
-                uint32_t d[4];
+                for (int st = 0; st < steps; ++st) {
+                    const uint4 k4 = key4(st);
+                    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+                    bool in[4], any = false;
+                    uint32_t d[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    in[e] = k[e] != 0 && k[e] - limit <= span;
-                    d[e] = (k[e] >> shift) & digits;
-                    any |= in[e];
-                }
-                if (!__ballot(any)) continue;
-                const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
-                if (!__ballot(!(in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 && d[2] == d0 && d[3] == d0))) {
-                    if (lane == 0) atomicAdd(&hist[d0], 4u * kWave);
-                    continue;
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        in[e] = k[e] != 0 && k[e] - limit <= span;
+                        d[e] = (k[e] >> shift) & digits;
+                        any |= in[e];
+                    }
+                    if (!__ballot(any)) continue;
+                    const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+                    if (!gather && !__ballot(!(in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 &&
+                                               d[2] == d0 && d[3] == d0))) {
+                        if (lane == 0) atomicAdd(&hist[d0], 4u * kWave);
+                        continue;
+                    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (in[e]) atomicAdd(&hist[d[e]], 1u);
+                    for (int e = 0; e < 4; ++e)
+                        if (in[e]) atomicAdd(&hist[d[e]], 1u);
+                    if (gather) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (in[e]) few[atomicAdd(&s_few, 1u)] = k[e];  // (at most `here` of them)
+                    }
+                }
             }
         }
         __syncthreads();
@@ -173,10 +214,13 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
             const bool first = need <= before + h1;
             s_digit = (unsigned)(kBins - (first ? 1 : 2) - 2 * tid);
             s_need = need - before - (first ? 0 : h1);
+            s_here = first ? h1 : h2;
         }
         __syncthreads();
         limit |= s_digit << shift;
         need = s_need;
+        if (pass == 0) here = s_here;
+        if (gather) n_few = s_few;
     }
     // `limit` is the smallest kept key now, and `need` of its equals stay
     unsigned n_larger = 0, n_equal = 0;  // in the segments before
@@ -400,13 +444,21 @@ extern "C" int jinf_cache_append(void* k_cache, void* v_cache, int kv_type, int6
         return JINF_HIP_ERR_INVALID;
     if (weights && (ld_w < max_ctx || (n_seq > 1 && ld_w_seq < n_heads_kv * ld_w)))
         return JINF_HIP_ERR_INVALID;
+    // 8 elements a thread where every row starts at 16 bytes, else one
+    const int64_t cs = kv_size(kv_type), rs = kv_size(rows_type);
+    const bool wide = kvw % 8 == 0 && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(k_rows, 16) &&
+                      aligned(v_rows, 16) && ld_pos * cs % 16 == 0 && ld_seq * cs % 16 == 0 &&
+                      ld_rows * rs % 16 == 0 && ld_rows_seq * rs % 16 == 0;
+    const int64_t units = wide ? kvw / 8 : kvw;
     // (no rows: one workgroup a sequence still writes its length)
-    const dim3 grid((unsigned)(n_take > 0 ? n_take : 1), (unsigned)n_seq);
-#define JINF_KV_APPEND(TC, TR)                                                                     \
-    launch(kv_append_kernel<TC, TR>, grid, dim3(kKvThreads), 0, stream, static_cast<TC*>(k_cache), \
-           static_cast<TC*>(v_cache), ld_pos, ld_seq, weights, ld_w, ld_w_seq, lens, lens_out,     \
-           static_cast<const TR*>(k_rows), static_cast<const TR*>(v_rows), ld_rows, ld_rows_seq,   \
-           n_rows, index, counts, n_take, max_ctx, (int)kvw, n_heads_kv)
+    const int64_t blocks = ((int64_t)n_take * 2 * units + kKvThreads - 1) / kKvThreads;
+    if (blocks > 0x7FFFFFFF) return JINF_HIP_ERR_INVALID;
+    const dim3 grid((unsigned)(blocks > 0 ? blocks : 1), (unsigned)n_seq);
+#define JINF_KV_APPEND(TC, TR)                                                                       \
+    launch(wide ? kv_append_kernel<TC, TR, 8> : kv_append_kernel<TC, TR, 1>, grid, dim3(kKvThreads), 0, \
+           stream, static_cast<TC*>(k_cache), static_cast<TC*>(v_cache), ld_pos, ld_seq, weights, ld_w, \
+           ld_w_seq, lens, lens_out, static_cast<const TR*>(k_rows), static_cast<const TR*>(v_rows),  \
+           ld_rows, ld_rows_seq, n_rows, index, counts, n_take, max_ctx, (int)units, n_heads_kv)
     if (kv_type == JINF_HIP_F16)
         return rows_type == JINF_HIP_F16 ? JINF_KV_APPEND(uint16_t, uint16_t)
                                          : JINF_KV_APPEND(uint16_t, float);
