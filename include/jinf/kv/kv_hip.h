@@ -55,8 +55,9 @@ extern "C" {
  * and to the drafted tokens j whose bit is set in its mask row:
  *   out[s, i, h] = sum softmax(scale * q[s,i,h] . k) v   over those rows,
  * kv head h / (n_heads / n_heads_kv).  A node with no row gets zeros, one with a
- * NaN score NaN.  A non-finite V value makes its dim NaN in the nodes that
- * attend to it, and in no other.
+ * NaN score NaN (an infinite key may make a score NaN).  A non-finite V value makes
+ * its dim non-finite in the nodes that attend to it; non-finite values in rows that a
+ * node does not attend to do not reach it.
  *   - q, out: fp32; node (s, i) at s * ld_q_seq + i * ld_q (ld_out alike).
  *   - k_draft, v_draft: the nodes' K (rotated to their positions) and V rows,
  *     (s, i) at s * ld_draft_seq + i * ld_draft, of draft_type F32 or F16; used

@@ -179,7 +179,7 @@ __device__ __forceinline__ void tr_split_exp(const float (&x)[4], float minus_on
     }
 }
 
-template <typename TC, int HD, int R_, int RW_, bool SCORE, bool ONCE>
+template <typename TC, int HD, int R_, int RW_, bool ONCE>
 struct TreeShape {
     static constexpr bool F16 = sizeof(TC) == 2;
     static constexpr int R = R_, RW = RW_, PW = 4 / RW_;
@@ -198,11 +198,7 @@ struct TreeShape {
     // 8192 with scores: 353 against 389 us; 6 fp32 sequences x 3001: 29.6 against 19.5).
     static constexpr int NS = ONCE && RW == 1 && BUF <= 32768 ? 4 : 2;
     static constexpr int MERGE = PW > 1 ? PW * ROWS * (HD + 4) * 4 : 0;
-    // A fifth wave that stores the scores, from two tiles' worth behind the tiles.
-    static constexpr bool STORER = SCORE && R == 1 && RW == 1;
-    static constexpr int THREADS = STORER ? 320 : 256;
-    static constexpr int TILES = NS * BUF > MERGE ? NS * BUF : MERGE;
-    static constexpr int LDS = TILES + (STORER ? 2 * ST * ROWS * 4 : 0);
+    static constexpr int LDS = NS * BUF > MERGE ? NS * BUF : MERGE;
     static constexpr int WGS = 2 * LDS <= 159 * 1024 ? 2 : 1;  // workgroups per CU
 };
 
@@ -229,10 +225,8 @@ __device__ __forceinline__ int tree_v_at(int r, int c) {
 // SCORE: one node a sequence, no drafted tokens, and the scores kept.
 // ONCE: the caches are read once and are larger than what the Infinity Cache keeps.
 template <typename TC, int HD, int R, int RW, bool SCORE, bool ONCE>
-__global__ __launch_bounds__((TreeShape<TC, HD, R, RW, SCORE, ONCE>::THREADS),
-                             (TreeShape<TC, HD, R, RW, SCORE, ONCE>::WGS))
-void tree_mfma_kernel(TreeArgs a) {
-    using Sh = TreeShape<TC, HD, R, RW, SCORE, ONCE>;
+__global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tree_mfma_kernel(TreeArgs a) {
+    using Sh = TreeShape<TC, HD, R, RW, ONCE>;
     constexpr bool F16 = Sh::F16;
     constexpr int PW = Sh::PW, ST = Sh::ST, TP = Sh::TP, PITCH = Sh::PITCH, CH = Sh::CH, LD = Sh::LD;
     constexpr int NS = Sh::NS;
@@ -317,29 +311,6 @@ void tree_mfma_kernel(TreeArgs a) {
     auto scores_at = [&](int p0) {
         return a.scores + (((int64_t)s * a.n_kv + j) * a.blocks + (p0 >> 4)) * a.group * 16;
     };
-    if constexpr (Sh::STORER) {
-        // The fifth wave stores each tile's scores one tile later.  (Stored by the waves
-        // that load, a store's answer holds up those of the loads behind it: 64
-        // sequences x 8192 positions 396 us, without stores 322.)
-        if (wave == 4) {
-            auto store = [&](int it) {
-                const int p0 = c0 + it * ST, n = min(ST, c1 - p0);
-                const float* from = reinterpret_cast<const float*>(tree_lds + Sh::TILES) + (it & 1) * ST * Sh::ROWS;
-                float* to = scores_at(p0);
-                for (int x = 4 * lane; x < (n + 15) / 16 * 16 * a.group; x += 4 * kWave)
-                    *reinterpret_cast<tr_f4*>(to + x) = *reinterpret_cast<const tr_f4*>(from + x);
-            };
-            for (int it = 0; it < n_it; ++it) {
-                __syncthreads();
-                if (it > 0) store(it - 1);
-            }
-            __syncthreads();
-            if (n_it > 0) store(n_it - 1);
-            __syncthreads();
-            return;
-        }
-    }
-
     const char* kb = reinterpret_cast<const char*>(static_cast<const TC*>(a.kc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
     const char* vb = reinterpret_cast<const char*>(static_cast<const TC*>(a.vc) + (int64_t)s * a.ld_seq + (int64_t)j * HD);
     const uint32_t rowb = (uint32_t)a.ld_pos * (uint32_t)sizeof(TC);  // (the host keeps ST of them below 2^31)
@@ -544,10 +515,9 @@ void tree_mfma_kernel(TreeArgs a) {
                                 if (16 * b + 4 * lg + r >= left) S[g][b][r] = -INFINITY;
                 }
                 if constexpr (SCORE) {
+                    // (Their 100 MB beside 1.6 GB read cost 64 x 8192 positions 40 us with loads past
+                    // the Infinity Cache, whichever wave stores them and in whatever bursts.)
                     float* to = scores_at(p0);
-                    if constexpr (Sh::STORER)
-                        to = reinterpret_cast<float*>(tree_lds + Sh::TILES) + (it & 1) * ST * Sh::ROWS +
-                             sub * a.group;
 #pragma unroll
                     for (int g = 0; g < R; ++g)
 #pragma unroll
@@ -881,16 +851,6 @@ constexpr int kTreeChunkMin = 128;  // positions per chunk, at least
 // nodes x 333 positions 17.5 against 15.6 us.)
 int tree_chunk_min(int wg_rows) { return wg_rows * 2 > kTreeChunkMin ? wg_rows * 2 : kTreeChunkMin; }
 
-// Rows of partial sums that calls of up to these sizes need: split calls have at
-// most tree_items workgroups.
-int64_t tree_part_rows(int n_seq, int max_nodes, int n_heads, int n_heads_kv, int max_ctx) {
-    const int64_t rows = (int64_t)max_nodes * (n_heads / n_heads_kv);
-    const int wr = tree_wg_rows(rows);
-    const int64_t a = (int64_t)kTreeItems * (wr <= 32 ? 4 : 1) * wr;
-    const int64_t b = (int64_t)n_seq * n_heads * max_nodes * ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
-    return a < b ? a : b;
-}
-
 // Caches that hold more than this are not expected in the Infinity Cache (256 MB) when
 // they are read again; where no two workgroups read the same rows either, K and V are
 // loaded past it, which leaves it to the scores and partial sums (64 sequences x 8192
@@ -902,23 +862,33 @@ bool tree_once(const TreeArgs& a, int kv_type, int n_seq) {
            (int64_t)n_seq * a.max_ctx * a.n_kv * a.head_dim * es * 2 > kTreeOnceBytes;
 }
 
-// Workgroups to aim for: what the chip holds at once (more add their own starts and
-// ends: 16 x 25 x 4096 70 us at 512, 78 at 1024), but four times as many where few
-// rows stream large caches, whose ragged ends then even out (64 x 8192 with scores, 389
-// us at 2048, 418 at 512).
-int64_t tree_items(const TreeArgs& a, int kv_type, int n_seq) {
-    return (int64_t)a.max_nodes * a.group <= 32 && tree_once(a, kv_type, n_seq) ? 4 * kTreeItems : kTreeItems;
+// Chunks per context: as many as make kTreeItems workgroups, what the chip holds at
+// once (more add their own starts and ends: 16 x 25 x 4096 70 us, 78 at twice as many;
+// 4 x 64 x 32768 419 either way).  Four times as many where few rows stream large
+// caches, whose ragged ends then even out (64 x 8192 with scores 418 -> 389 us).
+constexpr int kTreeMany = 4 * kTreeItems;
+int64_t tree_chunks(int64_t base, int wg_rows, bool stream_large, int max_ctx) {
+    const int cmin = tree_chunk_min(wg_rows);
+    const int64_t n = (stream_large ? kTreeMany : kTreeItems) / base;
+    const int64_t most = (max_ctx + cmin - 1) / cmin;
+    return n < most ? n : most;
 }
 
-// Splits contexts so that about kTreeItems workgroups share the call; rows of partial
-// sums used.
+// Rows of partial sums that calls of up to these sizes need.
+int64_t tree_part_rows(int n_seq, int max_nodes, int n_heads, int n_heads_kv, int max_ctx) {
+    const int wr = tree_wg_rows((int64_t)max_nodes * (n_heads / n_heads_kv));
+    const int64_t few = (int64_t)kTreeItems * wr, narrow = (int64_t)kTreeMany * (wr < 32 ? wr : 32);
+    const int64_t a = few > narrow ? few : narrow;
+    const int64_t b = (int64_t)n_seq * n_heads * max_nodes * ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
+    return a < b ? a : b;
+}
+
+// Splits contexts into chunks; rows of partial sums used.
 int64_t tree_plan(TreeArgs& a, int kv_type, int n_seq, int64_t part_rows) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int wr = tree_wg_rows(rows);
     const int64_t base = (int64_t)n_seq * a.n_kv * ((rows + wr - 1) / wr);
-    const int cmin = tree_chunk_min(wr);
-    int64_t nch = tree_items(a, kv_type, n_seq) / base;
-    if (nch > (a.max_ctx + cmin - 1) / cmin) nch = (a.max_ctx + cmin - 1) / cmin;
+    const int64_t nch = tree_chunks(base, wr, rows <= 32 && tree_once(a, kv_type, n_seq), a.max_ctx);
     a.chunk = a.max_ctx > 0 ? a.max_ctx : 1;
     a.nch = 1;
     if (nch > 1) {
@@ -939,12 +909,12 @@ bool tree_fast(const TreeArgs& a, int kv_type) {
 
 template <typename TC, int HD, int R, int RW, bool SCORE>
 int tree_launch(const TreeArgs& a, int n_seq, bool once, hipStream_t stream) {
-    using Sh = TreeShape<TC, HD, R, RW, SCORE, false>;
-    using Big = TreeShape<TC, HD, R, RW, SCORE, true>;
+    using Sh = TreeShape<TC, HD, R, RW, false>;
+    using Big = TreeShape<TC, HD, R, RW, true>;
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const dim3 grid((unsigned)((rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv), (unsigned)n_seq, (unsigned)a.nch);
-    return once ? launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, true>, grid, dim3(Big::THREADS), Big::LDS, stream, a)
-                : launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, false>, grid, dim3(Sh::THREADS), Sh::LDS, stream, a);
+    return once ? launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, true>, grid, dim3(256), Big::LDS, stream, a)
+                : launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, false>, grid, dim3(256), Sh::LDS, stream, a);
 }
 
 // SCORE: the scored decode, which joins the chunks' partial sums itself.

@@ -171,7 +171,7 @@ def cache_append(k_cache, v_cache, lens, k_rows, v_rows, n_heads_kv, index=None,
     _ints("lens_out", lens_out, n_seq)
     take = rows
     if index is not None:
-        take = index.shape[-1]
+        take = index.shape[1] if index.dim() == 2 else -1
         _ints("index", index, n_seq, take)
     if counts is not None:
         _ints("counts", counts, n_seq)

@@ -238,6 +238,49 @@ def test_tree_cache_past_32_bit_offsets(dev):
     close(host(w), ww, ww, "far positions' weights")
 
 
+@pytest.mark.parametrize("kv,ctx", [("f16", 17000), ("f32", 8500)])
+@pytest.mark.parametrize("T", [3, 10, 25, 50])
+def test_tree_large_caches(dev, kv, ctx, T):
+    """Caches past 128 MB, which take loads and tile counts of their own, at each number
+    of rows a workgroup holds (6 to 100 rows a kv head)."""
+    run_tree(2, T, ctx, 16, 8, 128, kv, "f32", [ctx, ctx // 2 + 1], n_nodes=[T, max(1, T // 2)])
+
+
+def test_tree_large_caches_of_narrow_heads(dev):
+    run_tree(2, 7, 17000, 32, 16, 64, "f16", "f16", [17000, 63])
+
+
+def test_one_workspace_for_calls_of_many_shapes(dev):
+    """A workspace of the largest shape serves smaller ones in any order, whatever it
+    held before; two calls on two streams, with one each, do not disturb each other."""
+    shapes = [(3, 30, 3000, 8, 2), (1, 3, 2999, 8, 2), (2, 64, 1500, 8, 2), (3, 1, 640, 8, 2)]
+    size = max(jinf_amd.attention_tree_workspace(n, T, nh, nk, 64, ctx).numel()
+               for n, T, ctx, nh, nk in shapes)
+    top = jinf_amd.attention_tree_workspace(3, 64, 8, 2, 64, 3000)
+    assert top.numel() >= size
+    top.fill_(255)
+    calls = []
+    for n, T, ctx, nh, nk in shapes:
+        k, v = (rand(i, n, ctx, nk * 64, dtype=torch.float16) for i in (1, 2))
+        q, kd, vd = rand(3, n, T, nh * 64), rand(4, n, T, nk * 64), rand(5, n, T, nk * 64)
+        mask = random_mask(np.random.default_rng(T), n, T)
+        lens = [ctx] * n
+        args = (q.cuda(), k.cuda(), v.cuda(), ints(lens), kd.cuda(), vd.cuda(), mask, nh, nk)
+        got = host(jinf_amd.attention_tree(*args, workspace=top)).copy()
+        want, mag = kv_ref.tree(q, k, v, lens, kd, vd, mask, nh, nk)
+        close(got, want, mag, f"shared workspace n={n} T={T} ctx={ctx}")
+        calls.append((args, got))
+    streams, outs = [torch.cuda.Stream() for _ in calls], []
+    spaces = [jinf_amd.attention_tree_workspace(n, T, nh, nk, 64, ctx) for n, T, ctx, nh, nk in shapes]
+    torch.cuda.synchronize()
+    for (args, _), st, ws in zip(calls, streams, spaces):
+        with torch.cuda.stream(st):
+            outs.append(jinf_amd.attention_tree(*args, workspace=ws))
+    torch.cuda.synchronize()
+    for (_, got), out in zip(calls, outs):
+        assert np.array_equal(host(out), got)
+
+
 # ---- one token with summed weights ----
 
 def run_scored(n, ctx, nh, nk, hd, kv, lens, pad=0, steps=2):
@@ -281,6 +324,13 @@ def test_scored_shapes(dev, n, ctx, nh, nk, hd, kv):
 @pytest.mark.parametrize("pad", [1, 8])
 def test_scored_lengths_and_strides(dev, kv, pad):
     run_scored(6, 200, 8, 2, 64, kv, [0, 1, 64, 65, -3, 500], pad=pad)
+
+
+@pytest.mark.parametrize("kv,ctx,nh,nk,hd", [("f16", 17000, 16, 8, 128), ("f32", 8500, 16, 8, 128),
+                                             ("f16", 17000, 160, 8, 128), ("f16", 17000, 64, 16, 64)])
+def test_scored_large_caches(dev, kv, ctx, nh, nk, hd):
+    """Caches past 128 MB, 2, 4 and 20 query heads a kv head."""
+    run_scored(2, ctx, nh, nk, hd, kv, [ctx, 4321], steps=1)
 
 
 @pytest.mark.parametrize("kv", list(DT))
