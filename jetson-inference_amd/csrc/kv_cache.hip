@@ -125,8 +125,12 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
             }
             uint32_t k[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                k[e] = at + e >= n ? 0u : t + e < n_first || t + e >= len - n_recent ? kKeyStays : weight_key(x[e]);
+            for (int e = 0; e < 4; ++e) k[e] = weight_key(x[e]);
+            if (__ballot(t < n_first || t + 4 > len - n_recent)) {  // (past the end, too)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    k[e] = t + e >= len ? 0u : t + e < n_first || t + e >= len - n_recent ? kKeyStays : k[e];
+            }
             *reinterpret_cast<uint4*>(keys + at) = make_uint4(k[0], k[1], k[2], k[3]);
         }
         __syncthreads();
@@ -160,7 +164,8 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digits = pass == 2 ? 1023u : 2047u;
-        // keys whose digits before are the threshold's lie in [limit, limit + span]
+        // keys whose digits before are the threshold's lie in [limit, limit + span] (0, no
+        // key, is counted in the first pass, below every key, where nobody looks)
         const uint32_t span = pass == 0 ? 0xFFFFFFFFu : pass == 1 ? (1u << 21) - 1 : 1023u;
         hist[tid] = 0, hist[tid + kSelThreads] = 0;
         if (pass == 0 && tid == 0) s_few = 0;
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
                     uint32_t d[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        in[e] = k[e] != 0 && k[e] - limit <= span;
+                        in[e] = k[e] - limit <= span;
                         d[e] = (k[e] >> shift) & digits;
                         any |= in[e];
                     }
@@ -232,8 +237,10 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
             const uint4 k = key4(st);
             const unsigned larger = __popcll(__ballot(k.x > limit)) + __popcll(__ballot(k.y > limit)) +
                                     __popcll(__ballot(k.z > limit)) + __popcll(__ballot(k.w > limit));
-            const unsigned equal = __popcll(__ballot(k.x == limit)) + __popcll(__ballot(k.y == limit)) +
-                                   __popcll(__ballot(k.z == limit)) + __popcll(__ballot(k.w == limit));
+            unsigned equal = 0;  // (few keys equal the threshold)
+            if (__ballot(k.x == limit || k.y == limit || k.z == limit || k.w == limit))
+                equal = __popcll(__ballot(k.x == limit)) + __popcll(__ballot(k.y == limit)) +
+                        __popcll(__ballot(k.z == limit)) + __popcll(__ballot(k.w == limit));
             if (lane == 0) counts[0][st * kWaves + wave] = larger, counts[1][st * kWaves + wave] = equal;
         }
         __syncthreads();
@@ -254,9 +261,15 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
             // the lanes before, then this lane's own four in turn
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const unsigned long long x = __ballot(k[e] > limit), y = __ballot(k[e] == limit);
+                const unsigned long long x = __ballot(k[e] > limit);
                 a = __builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, a));
-                b = __builtin_amdgcn_mbcnt_hi((uint32_t)(y >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)y, b));
+            }
+            if (__ballot(k[0] == limit || k[1] == limit || k[2] == limit || k[3] == limit)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned long long y = __ballot(k[e] == limit);
+                    b = __builtin_amdgcn_mbcnt_hi((uint32_t)(y >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)y, b));
+                }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
