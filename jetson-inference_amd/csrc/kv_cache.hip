@@ -75,10 +75,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // before it plus that of equals before it, at most as many as stay.
 //
 // What bounds it: instruction issue in the one workgroup, hence four keys a read and
-// no range checks, and few keys left for the last digit; and code size, hence the rolled loops (weights in registers with
-// unrolled passes, 50 KB of code, took 35 us at 8192 positions, fetching
-// instructions).  Weights of one magnitude meet in few counters: a wave whose keys
-// all share a digit adds once.
+// no range checks, and few keys left for the last digit; and code size, hence the
+// rolled loops (weights in registers with unrolled passes, 50 KB of code, took 35 us at
+// 8192 positions, fetching instructions).  Weights of one magnitude meet in few
+// counters: a wave whose keys all share a digit adds once.
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kBins = 2048;
 constexpr int kSelFew = 2048;  // keys that share the threshold's first digits, gathered if no more
@@ -285,10 +285,11 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(
 
 // The kept rows to their places: grid (n_kv slices, n_seq, 2 planes x chunks + 1), rows in
 // order, `w` units of a row a workgroup; the last of the third index move the weights
-// (by the workgroups of slice 0).  A kept row moves to a lower position or stays.  In place, one workgroup therefore walks all rows of its slice, and a
-// step's rows are all read before its first is written: rows that later steps read
-// lie past them, so the next step's loads are under way meanwhile.  Into other
-// caches, chunks of rows are independent.
+// (by the workgroups of slice 0).  A kept row moves to a lower position or stays.  In
+// place, one workgroup therefore walks all rows of its slice, and a step's rows are all
+// read before its first is written: rows that later steps read lie past them, so the
+// next step's loads are under way meanwhile.  Into other caches, chunks of rows are
+// independent.
 //
 // What bounds it: the rows' bytes, read and written once; with few sequences, how
 // many of them one workgroup keeps in flight (64 KiB here), hence the slices.
@@ -352,10 +353,11 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(
     if (is_weights && slice > 0) return;
     const int len = min(max(lens[s], 0), max_ctx);
     const int keep = min(len, budget);
-    // (lens_out may be lens: min(len, budget) is the same number before and after)
+    // (lens_out may be lens: min(len, budget) is the same number before and after, len is
+    // not, so what tells whether rows move is the last one's place: the list ascends)
     if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = keep;
-    if (in_place && len <= budget) return;
     const int32_t* at = list + ((int64_t)s * n_kv + j) * budget;
+    if (in_place && (keep == 0 || at[keep - 1] == keep - 1)) return;
     if (is_weights) {
         move_rows(weights_out + (int64_t)s * ld_wo_seq + (int64_t)j * ld_wo, 1,
                   weights + (int64_t)s * ld_w_seq + (int64_t)j * ld_w, 1, at, 0, keep, kMoveThreads,

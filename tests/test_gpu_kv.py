@@ -521,6 +521,25 @@ def test_evict_into_its_lengths(dev):
     assert host(lens).tolist() == [10, 4]
 
 
+def test_evict_into_its_lengths_with_many_workgroups(dev):
+    """More (sequence, kv head, plane) triples than run at once: those that start after a
+    sequence's new length is stored in place of its old one move its rows all the same."""
+    n, ctx, nk, hd, budget = 200, 600, 8, 64, 300
+    k, v = (rand(i, n, ctx, nk * hd, dtype=torch.float16).cuda() for i in (1, 2))
+    w = rand(3, n, nk, ctx).abs().cuda()
+    lens = ints([ctx - 2 * s for s in range(n)])
+    ko, vo = (torch.zeros(n, budget, nk * hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    wo = torch.zeros(n, nk, budget, device="cuda")
+    new = host(jinf_amd.cache_evict(k, v, w, lens, nk, budget, 4, 50, k_out=ko, v_out=vo, weights_out=wo))
+    say(f"evict in place into the lengths, {n} sequences")
+    jinf_amd.cache_evict(k, v, w, lens, nk, budget, 4, 50, lens_out=lens)
+    assert host(lens).tolist() == new.tolist() == [min(ctx - 2 * s, budget) for s in range(n)]
+    for s in range(n):
+        m = int(new[s])
+        assert torch.equal(k[s, :m], ko[s, :m]) and torch.equal(v[s, :m], vo[s, :m]), s
+        assert torch.equal(w[s, :, :m], wo[s, :, :m]), s
+
+
 # ---- together ----
 
 @pytest.mark.parametrize("kv", list(DT))
