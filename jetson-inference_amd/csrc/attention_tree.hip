@@ -29,13 +29,37 @@ struct TreeArgs {
     float* scores;  // null, or the scores wanted: [n_seq][n_kv][blocks][group][16], 16 positions a block
     int64_t blocks;
     int draft_f16;
-    // Contexts in chunks of `chunk` positions, nch of them at most; chunk 0 also
-    // takes the drafted tokens.  Row (s, j, r) chunk c has its partial sums at
-    // part[((s n_kv + j) rows + r) nch + c][head_dim] and {m, l} at stats[same].
+    // Contexts in chunks of `chunk` positions, nch of them at most, the first of which also
+    // takes the drafted tokens; each chunk of a row (s, j, r) has a record of partial sums
+    // part[rec][head_dim] and {m, l} stats[rec] (TreeRecords).
     int chunk, nch;
     float* part;
     float2* stats;
+    // Or, planned: chunks of `chunk` positions at least that the kernel divides itself
+    // (tree_share) into nch places per kv head, each a row tile's chunk and 2^planned
+    // records; a sequence's places follow each other, row tiles fastest.  It stores
+    // {first place, chunks, row tiles} of each of the n_seq sequences in front of part.
+    int n_seq, planned;
+    __device__ __forceinline__ int4* plan() const { return reinterpret_cast<int4*>(part) - n_seq; }
 };
+
+// Where the records of a kv head's rows are: row r's first at at(r), `step` apart.
+struct TreeRecords {
+    int64_t first;
+    int step, chunks, row_step, log;  // log: of the rows in a place
+    __device__ __forceinline__ int64_t at(int r) const {
+        return log < 0 ? first + (int64_t)r * row_step
+                       : first + ((int64_t)(r >> log) << log) + (r & ((1 << log) - 1));
+    }
+};
+__device__ __forceinline__ TreeRecords tree_records(const TreeArgs& a, int s, int j, int len) {
+    if (a.planned) {
+        const int4 p = a.plan()[s];
+        return {((int64_t)j * a.nch + p.x) << a.planned, p.z << a.planned, p.y, 1, a.planned};
+    }
+    return {((int64_t)s * a.n_kv + j) * a.max_nodes * a.group * a.nch, 1, max(1, (len + a.chunk - 1) / a.chunk),
+            a.nch, -1};
+}
 
 __device__ __forceinline__ float tree_exp2(float a) { return __builtin_amdgcn_exp2f(a); }
 
@@ -214,9 +238,64 @@ __device__ __forceinline__ int tree_v_at(int r, int c) {
     return c ^ (sizeof(TC) == 2 ? 2 * (r & 3) : 4 * ((r >> 2) & 3));
 }
 
-// grid (row tiles * n_kv, n_seq, chunks), 256 threads; the kv head is the fastest
-// index, so that row tiles of one head, which read the same K and V, lie n_kv
-// apart (on one XCD for 8 kv heads).  Heads, row tiles and sequences turn with the
+// Equal shares of ragged work, one lane a sequence (at most 64): the sequences' chunks,
+// of at most a common length, so that their row tiles' chunks fill the places.
+// Drafted tokens count as positions in front of a context.  The host knows neither
+// lengths nor node counts: chunks of the longest context possible leave workgroups
+// without work and the others with too much (4 sequences x 64 nodes, 16384 to 32768
+// positions: 403 -> 358 us; 64 x 1 with scores, 4096 to 8192: 373 -> 349).  Every
+// workgroup comes to the same division at its start, about a microsecond.
+struct TreeShare {
+    int s, tile, cix, chunks, tiles, first, chunk, ahead;  // chunk: positions, of which `ahead` before the context
+};
+template <int ROWS, bool SCORE>
+__device__ __forceinline__ bool tree_share(const TreeArgs& a, int place, TreeShare& w) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int at = min(lane, a.n_seq - 1);
+    const int held = a.lens[at], given = a.n_nodes ? a.n_nodes[at] : a.max_nodes;
+    const int len = min(max(held, 0), a.max_ctx);
+    const int nodes = lane < a.n_seq ? min(max(given, 0), a.max_nodes) : 0;
+    const int tiles = (nodes * a.group + ROWS - 1) / ROWS;
+    // in blocks of 64 positions, at least one
+    const int ahead = SCORE ? 0 : (nodes + 63) / 64;
+    const int v = max((len + 63) / 64 + ahead, 1);
+    // (guesses may round; the counts compared are whole numbers below 2^24)
+    const float all = wave_sum_f32((float)tiles * (float)v), least = wave_sum_f32((float)tiles);
+    int most = tiles ? v : 0;
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) most = max(most, __shfl_xor(most, o, kWave));
+    int c = max((int)ceilf(all / ((float)a.nch - 0.5f * least)), a.chunk / 64);
+    int n;
+    for (;;) {
+        n = (v + c - 1) / c;
+        // (one chunk each fits: the host counted places for the most row tiles)
+        if (c >= most || wave_sum_f32((float)(tiles * n)) <= (float)a.nch) break;
+        c += (c + 15) / 16;
+    }
+    const int chunk = (v + n - 1) / n;
+    n = (v + chunk - 1) / chunk;
+    int upto = tiles * n;  // places of the sequences before and this one
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) {
+        const int y = __shfl_up(upto, o, kWave);
+        if (lane >= o) upto += y;
+    }
+    const int s = __popcll(__ballot(upto <= place));
+    if (s >= a.n_seq) return false;
+    w.s = s;
+    w.chunks = __builtin_amdgcn_readlane(n, s);
+    w.tiles = __builtin_amdgcn_readlane(tiles, s);
+    w.first = __builtin_amdgcn_readlane(upto, s) - w.chunks * w.tiles;
+    w.chunk = __builtin_amdgcn_readlane(chunk, s) * 64;
+    w.ahead = __builtin_amdgcn_readlane(ahead, s) * 64;
+    w.cix = (place - w.first) / w.tiles;
+    w.tile = (place - w.first) % w.tiles;
+    return true;
+}
+
+// grid (row tiles * n_kv, n_seq, chunks), or (n_kv, places) where the kernel divides the
+// work (PLAN), 256 threads; the kv head is the fastest index, so that row tiles of one
+// head, which read the same K and V, lie n_kv apart (on one XCD for 8 kv heads).  Heads, row tiles and sequences turn with the
 // slower indices: workgroups go to XCDs, and in one of them to its 4 shader engines,
 // by their number in the grid, so that otherwise an XCD reads one head's addresses
 // alone (64 sequences x 8192, loads only: 335 -> 325 us) and the last, partly filled
@@ -224,7 +303,7 @@ __device__ __forceinline__ int tree_v_at(int r, int c) {
 // the time).
 // SCORE: one node a sequence, no drafted tokens, and the scores kept.
 // ONCE: the caches are read once and are larger than what the Infinity Cache keeps.
-template <typename TC, int HD, int R, int RW, bool SCORE, bool ONCE>
+template <typename TC, int HD, int R, int RW, bool SCORE, bool ONCE, bool PLAN>
 __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tree_mfma_kernel(TreeArgs a) {
     using Sh = TreeShape<TC, HD, R, RW, ONCE>;
     constexpr bool F16 = Sh::F16;
@@ -240,10 +319,18 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tr
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int col = lane & 15, lg = lane >> 4;
     const int pw = wave / RW, rw = wave % RW;
-    const int cix = blockIdx.z, s = (blockIdx.y + cix) % gridDim.y;
-    const int tile = (blockIdx.x / a.n_kv + blockIdx.y + cix) % (gridDim.x / a.n_kv);
-    const int j = (blockIdx.x + blockIdx.y + cix) % a.n_kv;
+    TreeShare w;
+    if constexpr (PLAN) {
+        if (!tree_share<Sh::ROWS, SCORE>(a, blockIdx.y, w)) return;
+    } else {
+        w.cix = blockIdx.z, w.s = (blockIdx.y + w.cix) % gridDim.y;
+        w.tile = (blockIdx.x / a.n_kv + blockIdx.y + w.cix) % (gridDim.x / a.n_kv);
+        w.chunk = a.chunk, w.ahead = 0;
+    }
+    const int s = w.s, cix = w.cix, tile = w.tile;
+    const int j = (blockIdx.x + (PLAN ? s : blockIdx.y) + cix) % a.n_kv;
     const int len = min(max(a.lens[s], 0), a.max_ctx);
+    if constexpr (!PLAN) w.chunks = max(1, (len + w.chunk - 1) / w.chunk);
     const int nodes = a.n_nodes ? min(max(a.n_nodes[s], 0), a.max_nodes) : a.max_nodes;
     const int rows = nodes * a.group, all_rows = a.max_nodes * a.group;
     const int row0 = tile * Sh::ROWS;
@@ -296,13 +383,14 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tr
             else asm volatile("" : "+v"(qf[g][u]));
         }
 
-    const int c0 = cix * a.chunk, c1 = min(len, c0 + a.chunk);
-    if (row0 >= rows || (cix > 0 && c0 >= len)) return;  // (workgroup-uniform, before any barrier)
+    const int c0 = max(cix * w.chunk - w.ahead, 0), c1 = min(len, (cix + 1) * w.chunk - w.ahead);
+    if (row0 >= rows || cix >= w.chunks) return;  // (workgroup-uniform, before any barrier)
+    if (PLAN && tile == 0 && cix == 0 && j == 0 && tid == 0)
+        a.plan()[s] = make_int4(w.first, w.chunks, w.tiles, 0);
     bool live[R];
 #pragma unroll
     for (int g = 0; g < R; ++g) live[g] = row0 + (rw * R + g) * 16 + col < rows;
     const bool idle = row0 + rw * R * 16 >= rows;  // none of the wave's rows is live
-    const int used = max(1, (len + a.chunk - 1) / a.chunk);
     const int drafts = !SCORE && cix == 0 ? nodes : 0;
     const int n_dt = (drafts + ST - 1) / ST;
     const int n_it = n_dt + (max(c1 - c0, 0) + ST - 1) / ST;
@@ -632,7 +720,7 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tr
         lsum[g] += __shfl_xor(lsum[g], 16, kWave);
         lsum[g] = xor32_sum(lsum[g]);
     }
-    const bool direct = used <= 1;
+    const bool direct = w.chunks <= 1;
     // Whether a node sees nothing at all: its outputs are zeros.  (A node whose
     // scores are all -inf has no sum either, and gets NaN.)
     auto sees_none = [&](int nd) {
@@ -644,17 +732,19 @@ __global__ __launch_bounds__(256, (TreeShape<TC, HD, R, RW, ONCE>::WGS)) void tr
         }
         return any == 0;
     };
-    // row r's place in the partial sums
-    const int64_t rec0 = ((int64_t)s * a.n_kv + j) * all_rows;
+    // row r's record of this chunk (TreeRecords)
+    const int64_t rec0 = PLAN ? ((int64_t)j * a.nch + w.first + cix * w.tiles + tile) * Sh::ROWS - row0
+                              : ((int64_t)s * a.n_kv + j) * all_rows;
+    auto rec = [&](int r) { return PLAN ? rec0 + r : (rec0 + r) * a.nch + cix; };
     auto put = [&](int r, int nd, int hh, int d, tr_f4 o, float M, float L) {
         if (direct) {
             float* p = a.out + (int64_t)s * a.ld_out_seq + (int64_t)nd * a.ld_out + (int64_t)hh * HD + d;
             const bool none = L == 0.0f && sees_none(nd);
             *reinterpret_cast<tr_f4u*>(p) = none ? tr_f4{0.f, 0.f, 0.f, 0.f} : o / L;
         } else {
-            *reinterpret_cast<tr_f4*>(a.part + ((rec0 + r) * a.nch + cix) * HD + d) = o;
+            *reinterpret_cast<tr_f4*>(a.part + rec(r) * HD + d) = o;
         }
-        if (d == 0 && a.stats) a.stats[(rec0 + r) * a.nch + cix] = make_float2(M, L);
+        if (d == 0 && a.stats) a.stats[rec(r)] = make_float2(M, L);
     };
     if constexpr (PW == 1) {
 #pragma unroll
@@ -706,25 +796,36 @@ template <int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     constexpr int LPR = HD / 4, RB = 256 / LPR;
     const int s = blockIdx.y, all_rows = a.max_nodes * a.group;
+    // (no plan is stored for a sequence without nodes)
     const int len = min(max(a.lens[s], 0), a.max_ctx);
-    const int used = (len + a.chunk - 1) / a.chunk;
-    if (used <= 1) return;
     const int nodes = a.n_nodes ? min(max(a.n_nodes[s], 0), a.max_nodes) : a.max_nodes;
     const int x = blockIdx.x * RB + threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
     const int j = x / all_rows, r = x % all_rows;
     if (j >= a.n_kv || r >= nodes * a.group) return;
-    const int64_t at = (((int64_t)s * a.n_kv + j) * all_rows + r) * a.nch;
-    float M = -INFINITY;
-    for (int c = 0; c < used; ++c) M = fmaxf(M, a.stats[at + c].x);
+    const TreeRecords recs = tree_records(a, s, j, len);
+    if (recs.chunks <= 1) return;
+    const int64_t at = recs.at(r);
+    const int step = recs.step;  // (all of a row's records lie within 2^18)
+    // a row's lanes share its chunks' {m, l} (one after the other: 6.5 us for 5 x 13 nodes
+    // x 12 chunks, 4.7 here)
+    const float2* st = a.stats + at;
+    const float* part = a.part + at * HD + d;
+    const int l = threadIdx.x % LPR;
+    float M = -INFINITY, L = 0.0f;
+    for (int c = l; c < recs.chunks; c += LPR) M = fmaxf(M, st[c * step].x);
+#pragma unroll
+    for (int o = 1; o < LPR; o *= 2) M = fmaxf(M, __shfl_xor(M, o, kWave));
     const float ref = softmax_ref(M);
-    tr_f4 o = {0.f, 0.f, 0.f, 0.f};
-    float L = 0.0f;
-    for (int c = 0; c < used; ++c) {
-        const float2 ml = a.stats[at + c];
-        const float f = tree_exp2(ml.x - ref);
-        L = fmaf(f, ml.y, L);
-        o += f * *reinterpret_cast<const tr_f4*>(a.part + (at + c) * HD + d);
+    for (int c = l; c < recs.chunks; c += LPR) {
+        const float2 ml = st[c * step];
+        L = fmaf(tree_exp2(ml.x - ref), ml.y, L);
     }
+#pragma unroll
+    for (int o = 1; o < LPR; o *= 2) L += __shfl_xor(L, o, kWave);
+    tr_f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int c = 0; c < recs.chunks; ++c)
+        o += tree_exp2(st[c * step].x - ref) * *reinterpret_cast<const tr_f4*>(part + c * step * HD);
     const int nd = r / a.group;
     float* p = a.out + (int64_t)s * a.ld_out_seq + (int64_t)nd * a.ld_out +
                (int64_t)(j * a.group + r - nd * a.group) * HD + d;
@@ -737,33 +838,35 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 // more where contexts are split, n_kv, n_seq); that last workgroup of each (sequence,
 // kv head) joins the outputs.
 // unit: what a probability of 1 counts in l.
-constexpr int kWtHeads = 64;  // heads whose {reference, unit / l} are held at a time
+constexpr int kWtHeads = 16;  // heads whose {reference, unit / l} are held at a time, 16 lanes each
 __global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ weights, int64_t ld_w,
                                                           int64_t ld_w_seq, TreeArgs a, float unit) {
     __shared__ float2 ml[kWtHeads];
     const int tid = threadIdx.x, j = blockIdx.y, s = blockIdx.z;
     const int len = min(max(a.lens[s], 0), a.max_ctx);
     const int t0 = blockIdx.x * 1024;
-    const int used = (len + a.chunk - 1) / a.chunk;
-    const int64_t h0 = (int64_t)s * a.n_heads + (int64_t)j * a.group;
-    if (a.nch > 1 && blockIdx.x == gridDim.x - 1) {
+    const TreeRecords recs = tree_records(a, s, j, len);
+    const int used = recs.chunks;
+    const int step = recs.step;
+    if (a.part && blockIdx.x == gridDim.x - 1) {
         if (used <= 1) return;
         const int hd = a.head_dim;
         for (int x = 4 * tid; x < a.group * hd; x += 1024) {
             const int g = x / hd, d = x % hd;
-            const float2* st = a.stats + (h0 + g) * a.nch;
+            const float2* st = a.stats + recs.at(g);
             float M = -INFINITY;
 #pragma unroll 4
-            for (int c = 0; c < used; ++c) M = fmaxf(M, st[c].x);
+            for (int c = 0; c < used; ++c) M = fmaxf(M, st[c * step].x);
             const float ref = softmax_ref(M);
-            const float* part = a.part + (h0 + g) * a.nch * hd + d;
+            const float* part = a.part + recs.at(g) * hd + d;
             tr_f4 o = {0.f, 0.f, 0.f, 0.f};
             float L = 0.0f;
 #pragma unroll 4
             for (int c = 0; c < used; ++c) {
-                const float f = tree_exp2(st[c].x - ref);
-                L = fmaf(f, st[c].y, L);
-                o += f * *reinterpret_cast<const tr_f4*>(part + (int64_t)c * hd);
+                const float2 x2 = st[c * step];
+                const float f = tree_exp2(x2.x - ref);
+                L = fmaf(f, x2.y, L);
+                o += f * *reinterpret_cast<const tr_f4*>(part + c * step * hd);
             }
             *reinterpret_cast<tr_f4u*>(a.out + (int64_t)s * a.ld_out_seq + ((int64_t)j * a.group + g) * hd + d) = o / L;
         }
@@ -774,19 +877,22 @@ __global__ __launch_bounds__(256) void tree_finish_kernel(float* __restrict__ we
     const int t = t0 + 4 * tid;
     for (int g0 = 0; g0 < a.group; g0 += kWtHeads) {
         const int n = min(kWtHeads, a.group - g0);
-        // 4 lanes a head share its chunks (in the order of the lanes)
-        const int g = tid >> 2, q4 = tid & 3;
+        // a head's lanes share its chunks
+        const int g = tid >> 4, l = tid & 15;
         if (g < n) {
-            const float2* st = a.stats + (h0 + g0 + g) * a.nch;
+            const float2* st = a.stats + recs.at(g0 + g);
             float M = -INFINITY, L = 0.0f;
-            for (int c = q4; c < used; c += 4) M = fmaxf(M, st[c].x);
-            M = fmaxf(M, dpp_f32<0xB1>(M));
-            M = fmaxf(M, dpp_f32<0x4E>(M));
+            for (int c = l; c < used; c += 16) M = fmaxf(M, st[c * step].x);
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) M = fmaxf(M, __shfl_xor(M, o, kWave));
             const float ref = softmax_ref(M);
-            for (int c = q4; c < used; c += 4) L = fmaf(tree_exp2(st[c].x - ref), st[c].y, L);
-            L += dpp_f32<0xB1>(L);
-            L += dpp_f32<0x4E>(L);
-            if (q4 == 0) ml[g] = make_float2(ref, unit / L);
+            for (int c = l; c < used; c += 16) {
+                const float2 x = st[c * step];
+                L = fmaf(tree_exp2(x.x - ref), x.y, L);
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) L += __shfl_xor(L, o, kWave);
+            if (l == 0) ml[g] = make_float2(ref, unit / L);
         }
         __syncthreads();
         if (t < len) {
@@ -866,7 +972,7 @@ bool tree_once(const TreeArgs& a, int kv_type, int n_seq) {
 
 // Chunks per context: as many as make kTreeItems workgroups, what the chip holds at
 // once (more add their own starts and ends: 16 x 25 x 4096 70 us, 78 at twice as many;
-// 4 x 64 x 32768 419 either way).  Four times as many where few rows stream large
+// 4 x 64 x 32768 in even chunks 419 either way).  Four times as many where few rows stream large
 // caches, whose ragged ends then even out (64 x 8192 with scores 418 -> 389 us).
 constexpr int kTreeMany = 4 * kTreeItems;
 int64_t tree_chunks(int64_t base, int wg_rows, bool stream_large, int max_ctx) {
@@ -876,29 +982,45 @@ int64_t tree_chunks(int64_t base, int wg_rows, bool stream_large, int max_ctx) {
     return n < most ? n : most;
 }
 
-// Rows of partial sums that calls of up to these sizes need.
+// Records of partial sums that calls of up to these sizes need.
 int64_t tree_part_rows(int n_seq, int max_nodes, int n_heads, int n_heads_kv, int max_ctx) {
-    const int wr = tree_wg_rows((int64_t)max_nodes * (n_heads / n_heads_kv));
+    const int64_t rows = (int64_t)max_nodes * (n_heads / n_heads_kv);
+    const int wr = tree_wg_rows(rows);
     const int64_t few = (int64_t)kTreeItems * wr, narrow = (int64_t)kTreeMany * (wr < 32 ? wr : 32);
     const int64_t a = few > narrow ? few : narrow;
-    const int64_t b = (int64_t)n_seq * n_heads * max_nodes * ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
+    const int64_t b = (int64_t)n_seq * n_heads_kv * ((rows + wr - 1) / wr) * wr *
+                      ((max_ctx + kTreeChunkMin - 1) / kTreeChunkMin + 1);
     return a < b ? a : b;
 }
 
-// Splits contexts into chunks; rows of partial sums used.
+bool tree_split(const TreeArgs& a) { return a.planned || a.nch > 1; }
+
+// Splits contexts into chunks, where the records fit into part_rows; records used.
+// The kernel divides the work itself (planned) where even chunks would have eight times
+// the fewest positions or more; below, its start costs what equal shares gain (16 x 25 x
+// 4096 69 to 72 us either way; 5 x 13 x 1999 31.3 planned, 29.6 not).
 int64_t tree_plan(TreeArgs& a, int kv_type, int n_seq, int64_t part_rows) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
-    const int wr = tree_wg_rows(rows);
+    const int wr = tree_wg_rows(rows), cmin = tree_chunk_min(wr);
     const int64_t base = (int64_t)n_seq * a.n_kv * ((rows + wr - 1) / wr);
-    const int64_t nch = tree_chunks(base, wr, rows <= 32 && tree_once(a, kv_type, n_seq), a.max_ctx);
-    a.chunk = a.max_ctx > 0 ? a.max_ctx : 1;
-    a.nch = 1;
+    const bool stream_large = rows <= 32 && tree_once(a, kv_type, n_seq);
+    const int64_t nch = tree_chunks(base, wr, stream_large, a.max_ctx);
+    const int items = stream_large ? kTreeMany : kTreeItems;
+    const int64_t places = items / a.n_kv;
+    a.n_seq = n_seq, a.chunk = a.max_ctx > 0 ? a.max_ctx : 1, a.nch = 1;
+    if (n_seq <= kWave && base <= items && nch > 0 && 8 * nch <= (a.max_ctx + cmin - 1) / cmin) {
+        if (places * a.n_kv * wr > part_rows) return 0;
+        a.nch = (int)places, a.chunk = cmin;
+        a.planned = wr == 16 ? 4 : wr == 32 ? 5 : wr == 64 ? 6 : 7;
+        return places * a.n_kv * wr;
+    }
+    const int64_t whole = (int64_t)n_seq * a.n_heads * a.max_nodes;
     if (nch > 1) {
         const int chunk = (int)((a.max_ctx + nch - 1) / nch + 63) / 64 * 64;
         const int n = (a.max_ctx + chunk - 1) / chunk;
-        if (n > 1 && (int64_t)n_seq * a.n_heads * a.max_nodes * n <= part_rows) a.chunk = chunk, a.nch = n;
+        if (n > 1 && whole * n <= part_rows) a.chunk = chunk, a.nch = n;
     }
-    return (int64_t)n_seq * a.n_heads * a.max_nodes * a.nch;
+    return tree_split(a) ? whole * a.nch : 0;
 }
 
 bool tree_fast(const TreeArgs& a, int kv_type) {
@@ -909,25 +1031,30 @@ bool tree_fast(const TreeArgs& a, int kv_type) {
            a.ld_pos * es <= (1 << 23);  // a tile's positions within 32-bit offsets
 }
 
-template <typename TC, int HD, int R, int RW, bool SCORE>
-int tree_launch(const TreeArgs& a, int n_seq, bool once, hipStream_t stream) {
-    using Sh = TreeShape<TC, HD, R, RW, false>;
-    using Big = TreeShape<TC, HD, R, RW, true>;
+template <typename TC, int HD, int R, int RW, bool SCORE, bool ONCE>
+int tree_launch(const TreeArgs& a, int n_seq, hipStream_t stream) {
+    using Sh = TreeShape<TC, HD, R, RW, ONCE>;
+    if (a.planned)
+        return launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, ONCE, true>, dim3((unsigned)a.n_kv, (unsigned)a.nch),
+                      dim3(256), Sh::LDS, stream, a);
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const dim3 grid((unsigned)((rows + Sh::ROWS - 1) / Sh::ROWS * a.n_kv), (unsigned)n_seq, (unsigned)a.nch);
-    return once ? launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, true>, grid, dim3(256), Big::LDS, stream, a)
-                : launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, false>, grid, dim3(256), Sh::LDS, stream, a);
+    return launch(tree_mfma_kernel<TC, HD, R, RW, SCORE, ONCE, false>, grid, dim3(256), Sh::LDS, stream, a);
 }
 
 // SCORE: the scored decode, which joins the chunks' partial sums itself.
 template <typename TC, int HD, bool SCORE>
 int tree_rows_launch(const TreeArgs& a, int n_seq, bool once, hipStream_t stream) {
     const int wr = tree_wg_rows((int64_t)a.max_nodes * a.group);
-    const int rc = wr == 16   ? tree_launch<TC, HD, 1, 1, SCORE>(a, n_seq, once, stream)
-                   : wr == 32 ? tree_launch<TC, HD, 2, 1, SCORE>(a, n_seq, once, stream)
-                   : wr == 64 ? tree_launch<TC, HD, 2, 2, SCORE>(a, n_seq, once, stream)
-                              : tree_launch<TC, HD, 2, 4, SCORE>(a, n_seq, once, stream);
-    if (rc != JINF_HIP_OK || a.nch <= 1 || SCORE) return rc;
+#define JINF_TREE_LAUNCH(R, RW)                                       \
+    (once ? tree_launch<TC, HD, R, RW, SCORE, true>(a, n_seq, stream) \
+          : tree_launch<TC, HD, R, RW, SCORE, false>(a, n_seq, stream))
+    const int rc = wr == 16   ? JINF_TREE_LAUNCH(1, 1)
+                   : wr == 32 ? JINF_TREE_LAUNCH(2, 1)
+                   : wr == 64 ? JINF_TREE_LAUNCH(2, 2)
+                              : JINF_TREE_LAUNCH(2, 4);
+#undef JINF_TREE_LAUNCH
+    if (rc != JINF_HIP_OK || !tree_split(a) || SCORE) return rc;
     constexpr int RB = 256 / (HD / 4);
     const int64_t all = (int64_t)a.max_nodes * a.group * a.n_kv;
     return launch(tree_merge_kernel<HD>, dim3((unsigned)((all + RB - 1) / RB), (unsigned)n_seq), dim3(256), 0,
@@ -952,8 +1079,8 @@ extern "C" size_t jinf_attention_tree_workspace_bytes(int n_seq, int max_nodes, 
     if (n_seq <= 0 || max_nodes <= 0 || n_heads <= 0 || n_heads_kv <= 0 || head_dim <= 0 || max_ctx < 0)
         return 0;
     if (n_heads % n_heads_kv != 0 || max_nodes > JINF_HIP_MAX_NODES) return 0;
-    // {m, l} and the sums of each row
-    return (size_t)jinf::tree_part_rows(n_seq, max_nodes, n_heads, n_heads_kv, max_ctx) *
+    // plan; sums and {m, l} of each record
+    return (size_t)n_seq * sizeof(int4) + (size_t)jinf::tree_part_rows(n_seq, max_nodes, n_heads, n_heads_kv, max_ctx) *
            (head_dim + 2) * sizeof(float) + 16;
 }
 
@@ -994,14 +1121,14 @@ extern "C" int jinf_attention_tree(float* out, int ld_out, int64_t ld_out_seq, c
     a.max_nodes = max_nodes, a.words = (max_nodes + 63) / 64, a.max_ctx = max_ctx;
     a.head_dim = head_dim, a.n_heads = n_heads, a.n_kv = n_heads_kv, a.group = n_heads / n_heads_kv;
     a.c = scale * kLog2e, a.draft_f16 = draft_type == JINF_HIP_F16;
-    a.chunk = max_ctx > 0 ? max_ctx : 1, a.nch = 1;
     if (!tree_fast(a, kv_type)) return tree_any(a, kv_type, n_seq, stream);
-    // workspace: the sums of as many rows as fit, then {m, l}
-    const int64_t fit = workspace && workspace_bytes > 16
-                            ? (int64_t)((workspace_bytes - 16) / ((head_dim + 2) * sizeof(float))) : 0;
+    // workspace: the plan, sums, {m, l}
+    const size_t plan_bytes = (size_t)n_seq * sizeof(int4);
+    const int64_t fit = workspace && workspace_bytes > plan_bytes
+                            ? (int64_t)((workspace_bytes - plan_bytes) / ((head_dim + 2) * sizeof(float))) : 0;
     const int64_t used = tree_plan(a, kv_type, n_seq, fit);
-    if (a.nch > 1) {
-        a.part = static_cast<float*>(workspace);
+    if (tree_split(a)) {
+        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes);
         a.stats = reinterpret_cast<float2*>(a.part + used * head_dim);
     }
     return tree_mfma<false>(a, kv_type, n_seq, stream);
@@ -1011,8 +1138,9 @@ extern "C" size_t jinf_attention_scored_workspace_bytes(int n_seq, int n_heads, 
                                                         int head_dim, int max_ctx) {
     if (n_seq <= 0 || n_heads <= 0 || n_heads_kv <= 0 || head_dim <= 0 || max_ctx < 0) return 0;
     if (n_heads % n_heads_kv != 0) return 0;
-    // scores, {m, l} of each row's one chunk at least, sums
-    return ((size_t)n_seq * n_heads * (16 * jinf::score_blocks(max_ctx) + 2) +
+    // scores, plan, {m, l} of one chunk a context at least, or sums and {m, l}
+    return ((size_t)n_seq * n_heads * 16 * jinf::score_blocks(max_ctx) + 4 * (size_t)n_seq +
+            2 * (size_t)n_seq * n_heads +
             (size_t)jinf::tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx) * (head_dim + 2)) *
                sizeof(float) + 16;
 }
@@ -1049,15 +1177,16 @@ extern "C" int jinf_attention_decode_scored(float* out, int ld_out, const float*
     a.n_heads = n_heads, a.n_kv = n_heads_kv, a.group = n_heads / n_heads_kv;
     a.c = scale * kLog2e;
     a.scores = static_cast<float*>(workspace), a.blocks = score_blocks(max_ctx);
+    float* part = a.scores + (int64_t)n_seq * n_heads * a.blocks * 16 + 4 * (int64_t)n_seq;  // (behind the plan)
     a.chunk = max_ctx > 0 ? max_ctx : 1, a.nch = 1;
-    a.part = a.scores + (int64_t)n_seq * n_heads * a.blocks * 16;
     const bool fast = tree_fast(a, kv_type);
-    int64_t used = (int64_t)n_seq * n_heads;
+    int64_t used = 0;
     if (fast) used = tree_plan(a, kv_type, n_seq, tree_part_rows(n_seq, 1, n_heads, n_heads_kv, max_ctx));
-    a.stats = reinterpret_cast<float2*>(a.part + (a.nch > 1 ? used * head_dim : 0));
+    if (tree_split(a)) a.part = part;
+    a.stats = reinterpret_cast<float2*>(part + (a.part ? used * head_dim : 0));
     rc = fast ? tree_mfma<true>(a, kv_type, n_seq, stream) : tree_any(a, kv_type, n_seq, stream);
     if (rc != JINF_HIP_OK || max_ctx == 0) return rc;
-    return launch(tree_finish_kernel, dim3((unsigned)((max_ctx + 1023) / 1024 + (a.nch > 1 ? 1 : 0)), (unsigned)n_heads_kv,
+    return launch(tree_finish_kernel, dim3((unsigned)((max_ctx + 1023) / 1024 + (a.part ? 1 : 0)), (unsigned)n_heads_kv,
                                            (unsigned)n_seq),
                   dim3(256), 0, stream, weights, ld_w, ld_w_seq, a, fast ? exp2f(kTreeUnit) : 1.0f);
 }

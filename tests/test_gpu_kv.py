@@ -250,6 +250,53 @@ def test_tree_large_caches_of_narrow_heads(dev):
     run_tree(2, 7, 17000, 32, 16, 64, "f16", "f16", [17000, 63])
 
 
+@pytest.mark.parametrize("n,T,ctx,nh,kv,lens,n_nodes", [
+    (5, 20, 14000, 16, "f16", [14000, 0, 1, 137, 9000], [20, 20, 0, 7, 13]),
+    (5, 20, 14000, 16, "f16", [40, 0, 0, 0, 0], [20, 3, 1, 0, 20]),
+    (5, 20, 14000, 16, "f16", [0, 14000, 14000, 14000, 14000], [0, 20, 20, 20, 20]),
+    (2, 256, 33000, 8, "f16", [300, 10000], [256, 70]),
+    (3, 20, 24000, 16, "f32", [24000, 640, 5], None),
+    (8, 3, 33000, 16, "f16", [33000, 0, 5, 12000, 700, 64, 2000, 1], [3, 3, 1, 2, 0, 3, 1, 3]),
+])
+def test_tree_ragged_work_in_equal_shares(dev, n, T, ctx, nh, kv, lens, n_nodes):
+    """Caches much longer than most contexts, sequences of many and no nodes: work that
+    the kernel divides by the lengths and counts it finds."""
+    run_tree(n, T, ctx, nh, 8, 64, kv, "f32", lens, n_nodes=n_nodes)
+
+
+def test_tree_shares_follow_the_lengths_of_each_replay(dev):
+    """One captured call, replayed as lengths and node counts change."""
+    n, T, ctx, nh, nk, hd = 5, 20, 14000, 16, 8, 64
+    k, v = (rand(i, n, ctx, nk * hd, dtype=torch.float16).cuda() for i in (1, 2))
+    q, kd, vd = rand(3, n, T, nh * hd).cuda(), rand(4, n, T, nk * hd).cuda(), rand(5, n, T, nk * hd).cuda()
+    mask = random_mask(np.random.default_rng(7), n, T)
+    lens, nodes = ints([14000] * n), ints([T] * n)
+    ws = jinf_amd.attention_tree_workspace(n, T, nh, nk, hd, ctx)
+    out = torch.zeros(n, T, nh * hd, device=dev)
+    args = (q, k, v, lens, kd, vd, mask, nh, nk, nodes)
+    jinf_amd.attention_tree(*args, out=out, workspace=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        jinf_amd.attention_tree(*args, out=out, workspace=ws)
+    for step, (a, b) in enumerate([([14000] * 5, [20] * 5), ([1, 14000, 0, 333, 7000], [20, 1, 5, 0, 19]),
+                                   ([0] * 5, [0, 0, 0, 0, 20]), ([9000, 9001, 64, 63, 2], [3] * 5)]):
+        lens.copy_(ints(a)), nodes.copy_(ints(b))
+        out.fill_(-3.0)
+        torch.cuda.synchronize()
+        g.replay()
+        got = host(out).copy()
+        torch.cuda.synchronize()
+        say(f"replay {step} of lengths {a}, nodes {b}")
+        want = torch.full_like(out, -3.0)
+        jinf_amd.attention_tree(*args, out=want, workspace=ws.clone())
+        assert np.array_equal(got, host(want)), step
+        whole = torch.full_like(out, -3.0)  # every context in one piece
+        jinf_amd.attention_tree(*args, out=whole, workspace=torch.empty(16, dtype=torch.uint8, device=dev))
+        top = v.float().abs().max().item()  # both within 2e-5 sum p |v| of the exact result
+        assert np.all(np.abs(got - host(whole)) <= 4e-5 * max(top, vd.abs().max().item())), step
+
+
 def test_one_workspace_for_calls_of_many_shapes(dev):
     """A workspace of the largest shape serves smaller ones in any order, whatever it
     held before; two calls on two streams, with one each, do not disturb each other."""
@@ -331,6 +378,11 @@ def test_scored_lengths_and_strides(dev, kv, pad):
 def test_scored_large_caches(dev, kv, ctx, nh, nk, hd):
     """Caches past 128 MB, 2, 4 and 20 query heads a kv head."""
     run_scored(2, ctx, nh, nk, hd, kv, [ctx, 4321], steps=1)
+
+
+@pytest.mark.parametrize("lens", [[33000, 0, 5, 12000, 700, 64, 2000, 1], [0] * 7 + [130]])
+def test_scored_ragged_work_in_equal_shares(dev, lens):
+    run_scored(8, 33000, 16, 8, 64, "f16", lens, steps=1)
 
 
 @pytest.mark.parametrize("kv", list(DT))
